@@ -159,6 +159,73 @@ bool tm_cuda_attn_decode_static_dev(const float* q, const void* kc, const void* 
                                     unsigned KVH, unsigned dh, unsigned ctx, unsigned allow, float scale,
                                     int kv_half, void* stream);
 
+/* ---- a batch of sequences (no counterpart in the reference, which decodes one sequence from one contiguous cache) -----------
+ * A serving step: tm_cuda_kv_append_paged_dev puts the new tokens' keys and values into the pages, tm_cuda_attn_paged_dev attends
+ * over them, tm_cuda_logits_rules_dev applies what the requests ask of the logits before a token is chosen
+ * (tm_cuda_argmax_dev). tm_cuda_attn_window_dev is the attention of one sequence over a contiguous cache.
+ *
+ * Sequence b has the rows [q_begin[b], q_begin[b + 1]) of q, qkv and out; they are its newest tokens, at the positions
+ * kv_len[b] - n .. kv_len[b] - 1 (kv_len counts them). Rows behind q_begin[B] are left as they are. Position p lies in row
+ * p % page of page table[b * table_ld + p / page]; entries that no position needs may hold anything. All arrays are device memory
+ * of the library's device, read when the kernels run: a captured graph may be replayed with other contents. The calls refuse what
+ * the host can see. What only the device sees is checked there: a page, length or range of rows that is out of range is
+ * not read or written, the rows of out that depend on it are NaN (rows that belong to no sequence: left as they are), and
+ * the next synchronising entry of the lane reports it. A new token before position 0 (more new tokens than kv_len says) is not stored,
+ * and sees no key.
+ * No call allocates or synchronises. Calls may run at the same time on several streams if each has its own scratch; a graph
+ * keeps using the scratch that it was captured with. */
+typedef struct tm_cuda_kv_pages {
+    void* k;                     /* [npages][KVH][page][dh], half when kv_half != 0, else fp32; on 16-byte boundaries */
+    void* v;
+    const int* table;            /* [B][table_ld] */
+    const int* q_begin;          /* [B + 1], ascending from 0 */
+    const int* kv_len;           /* [B] */
+    unsigned B, KVH, dh;         /* dh: a multiple of 8, at most 128 */
+    unsigned page, npages, table_ld;
+    int kv_half;
+} tm_cuda_kv_pages;
+/* qkv: [T][(H + 2 KVH) * dh] fp32, the new tokens' un-rotated q | k | v. q ([T][H * dh]) receives the rotated queries; rotated keys
+ * and values go into the pages (rounded once for half). rope: (cos, sin) pairs [rope_rows][dh / 2] for the pairs (j, j + dh/2) of a
+ * head, or NULL for none; a position behind the table is treated as a length out of range. q must not overlap qkv. Two sequences
+ * that share a page write to it in no order. */
+bool tm_cuda_kv_append_paged_dev(const tm_cuda_kv_pages* kv, const float* qkv, float* q, unsigned T, unsigned H, const float* rope,
+                                 unsigned rope_rows, void* stream);
+/* out[t] = softmax(scale q k) v over the keys j that the position p of token t sees: j <= p, and with window > 0 also
+ * j > p - window or j < sinks. A token that sees none: zeros. q, out: [T][H * dh] fp32; sums and statistics in fp32, results as from
+ * fp32 products with both cache types. max_q: the most new tokens that one sequence has (0: not known, T); a sequence with more is
+ * treated as out of range. `scratch` holds tm_cuda_attn_paged_scratch(...) bytes; what it holds before does not matter. */
+size_t tm_cuda_attn_paged_scratch(unsigned T, unsigned B, unsigned max_q, unsigned H, unsigned KVH, unsigned dh);
+bool tm_cuda_attn_paged_dev(const tm_cuda_kv_pages* kv, const float* q, float* scratch, size_t scratch_bytes, float* out, unsigned T,
+                            unsigned max_q, unsigned H, unsigned window, unsigned sinks, float scale, void* stream);
+/* The same for T tokens at positions pos0 .. pos0 + T - 1 of one sequence whose caches are [KVH][ctx][dh], as
+ * tm_cuda_attn_decode_dev has them; their keys and values are in the caches already. */
+size_t tm_cuda_attn_window_scratch(unsigned T, unsigned H, unsigned KVH, unsigned dh);
+bool tm_cuda_attn_window_dev(const float* q, const void* kc, const void* vc, float* scratch, size_t scratch_bytes, float* out,
+                             unsigned T, unsigned pos0, unsigned H, unsigned KVH, unsigned dh, unsigned ctx, unsigned window,
+                             unsigned sinks, float scale, int kv_half, void* stream);
+/* Rules on the logits x [B][ldx], V of each row, into out [B][ldo] (which may be x with the same stride, but not overlap it
+ * otherwise). In this order, each where its pointers are not NULL:
+ *   repeat     a token of the row's list: x > 0 ? x / repeat[b] : x * repeat[b]
+ *   frequency, presence   one that occurs c > 0 times in the list behind its first n_prompt[b] entries: x -= frequency[b] * c + presence[b]
+ *   bias       x[bias_ids[i]] += bias[i], for the first n_bias[b] entries (NULL: all bias_ld); of an id that is listed twice the last one
+ *   mask       -infinity where bit t % 32 of word t / 32 of the row's mask is 0
+ * Ids outside the vocabulary are skipped, lengths are cut to [0, stride]. B <= 65535. */
+typedef struct tm_cuda_logit_rules {
+    const int* tokens;           /* [B][tokens_ld]: prompt and generated tokens; n_tokens[b] of them count */
+    const int* n_tokens;
+    const int* n_prompt;         /* NULL: 0 */
+    const float* repeat;         /* [B] each */
+    const float* presence;
+    const float* frequency;
+    const int* bias_ids;         /* [B][bias_ld] */
+    const float* bias;
+    const int* n_bias;
+    const uint32_t* mask;        /* [B][mask_ld], mask_ld >= ceil(V / 32) */
+    unsigned tokens_ld, bias_ld, mask_ld;
+} tm_cuda_logit_rules;
+bool tm_cuda_logits_rules_dev(const float* x, size_t ldx, float* out, size_t ldo, unsigned B, unsigned V,
+                              const tm_cuda_logit_rules* rules, void* stream);
+
 /* ---- token lane (metal_shim.mm:22-152) ----------------------------------- */
 /* Slots are backend-owned grow-only device buffers addressed by small integers
  * (metal.h:2262-2281). A slot may not grow between tok_begin and the matching

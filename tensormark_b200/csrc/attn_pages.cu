@@ -1,0 +1,128 @@
+// attn_pages.cu — attention of the new tokens of a batch of sequences over a paged K/V cache, and of a chunk of tokens over a
+// contiguous one, with an optional sliding window and first tokens that stay visible. The simple form: a warp per query row.
+#include "cuda_shim.h"
+#include "common.cuh"
+#include "kv_pages.cuh"
+#include "state.h"
+
+#include <cmath>
+#include <cuda_fp16.h>
+#include <math_constants.h>
+
+namespace tmc {
+
+bool on_library_device(const char* who) {
+    if (!ensure_init(-1)) return false;
+    int dev = -1;
+    if (cudaGetDevice(&dev) == cudaSuccess && dev == state().device) return true;
+    cudaGetLastError();
+    return fail("%s: the library's device %d is not the current one", who, state().device);
+}
+
+bool kv_batch_from(KvBatch* c, const tm_cuda_kv_pages* kv, unsigned T, unsigned H, const char* who) {
+    if (!kv) return fail("%s: null pointer", who);
+    if (!kv->k || !kv->v || !kv->table || !kv->q_begin || !kv->kv_len) return fail("%s: null pointer in the cache's description", who);
+    if (!kv->B || !kv->KVH || !kv->page || !kv->npages || !kv->table_ld) return fail("%s: a zero in the cache's description", who);
+    if (!H || H % kv->KVH || H / kv->KVH > 128) return fail("%s: %u query heads for %u K/V heads (a multiple, at most 128 each)", who, H, kv->KVH);
+    if (!kv->dh || kv->dh % 8 || kv->dh > 128) return fail("%s: head dimension %u (multiples of 8 up to 128)", who, kv->dh);
+    if ((uintptr_t)kv->k % 16 || (uintptr_t)kv->v % 16) return fail("%s: the pages lie on 16-byte boundaries", who);
+    if ((unsigned long long)kv->table_ld * kv->page > 0x7fffffffull || T > 0x7fffffffu || kv->B > 0x7ffffffu) return fail("%s: more than 2^31 - 1 positions or tokens", who);
+    *c = KvBatch{kv->k, kv->v, kv->table, kv->q_begin, kv->kv_len, kv->B, kv->KVH, kv->dh, kv->page, kv->npages, kv->table_ld, T, kv->table_ld * kv->page, 0u, -1};
+    if ((kv->page & (kv->page - 1u)) == 0)
+        for (c->page_shift = 0; 1u << c->page_shift < kv->page;) ++c->page_shift;
+    return true;
+}
+
+namespace {
+
+template <typename T>
+__global__ void __launch_bounds__(128) attn_rows_kernel(KvBatch c, KvMask mask, const float* q, float* out, uint32_t H, uint32_t max_q, float scale, int* status) {
+    const uint32_t lane = threadIdx.x & 31u, id = blockIdx.x * 4u + (threadIdx.x >> 5), t = id / H, head = id % H;
+    if (t >= c.T) return;
+    const uint32_t b = kv_find_seq(c, t);
+    if (b >= c.B) return;
+    const KvSeq s = kv_seq(c, b);
+    if (s.lost || t < s.q0 || t - s.q0 >= s.n) { note_bad_batch(status); return; }
+    const uint32_t dh = c.dh;
+    const int p = s.first + (int)(t - s.q0);
+    const KvSpan span = kv_span(mask, p, p);
+    const T* kb = (const T*)c.k + (size_t)(head / (H / c.KVH)) * c.page * dh;
+    const T* vb = (const T*)c.v + (size_t)(head / (H / c.KVH)) * c.page * dh;
+    float qr[4], acc[4] = {}, m = -CUDART_INF_F, l = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) qr[i] = lane + 32u * i < dh ? q[((size_t)t * H + head) * dh + lane + 32u * i] * (scale * kLog2e) : 0.f;
+    bool bad = s.bad || s.n > max_q;
+    for (uint32_t j = span.a ? 0u : span.b; j < span.e; j = j + 1 == span.a ? span.b : j + 1) {
+        size_t at;
+        if (!kv_row(c, b, j, &at)) { bad = true; continue; }
+        float x = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (lane + 32u * i < dh) x = fmaf(qr[i], (float)kb[at + lane + 32u * i], x);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+        const float mn = fmaxf(m, x), corr = m == -CUDART_INF_F ? 0.f : exp2f(m - mn), w = x == -CUDART_INF_F ? 0.f : exp2f(x - mn + kUp);
+        l = fmaf(l, corr, w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (lane + 32u * i < dh) acc[i] = fmaf(acc[i], corr, w * (float)vb[at + lane + 32u * i]);
+        m = mn;
+    }
+    if (bad) { note_bad_batch(status); l = CUDART_NAN_F; }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (lane + 32u * i < dh) out[((size_t)t * H + head) * dh + lane + 32u * i] = l == 0.f ? 0.f : acc[i] / l;
+}
+
+bool launch(const KvBatch& c, KvMask mask, bool half, const float* q, float* out, unsigned H, unsigned max_q, float scale, cudaStream_t st) {
+    const size_t rows = (size_t)c.T * H;
+    if (rows > 0x7fffffffull) return fail("attention: %zu query rows", rows);
+    const unsigned grid = (unsigned)((rows + 3) / 4);
+    if (half) attn_rows_kernel<__half><<<grid, 128, 0, st>>>(c, mask, q, out, H, max_q, scale, device_status_word());
+    else attn_rows_kernel<float><<<grid, 128, 0, st>>>(c, mask, q, out, H, max_q, scale, device_status_word());
+    note_launch();
+    return check_launch("attention");
+}
+
+}  // namespace
+}  // namespace tmc
+
+using namespace tmc;
+
+extern "C" {
+
+size_t tm_cuda_attn_paged_scratch(unsigned T, unsigned B, unsigned max_q, unsigned H, unsigned KVH, unsigned dh) { return 256; }
+size_t tm_cuda_attn_window_scratch(unsigned T, unsigned H, unsigned KVH, unsigned dh) { return tm_cuda_attn_paged_scratch(T, 1, T, H, KVH, dh); }
+
+bool tm_cuda_attn_paged_dev(const tm_cuda_kv_pages* kv, const float* q, float* scratch, size_t scratch_bytes, float* out, unsigned T, unsigned max_q,
+                            unsigned H, unsigned window, unsigned sinks, float scale, void* stream) {
+    KvBatch c;
+    if (!kv_batch_from(&c, kv, T, H, "attn_paged")) return false;
+    if (!q || !out || !scratch) return fail("attn_paged: null pointer");
+    if ((uintptr_t)q % 16 || (uintptr_t)out % 16 || (uintptr_t)scratch % 16) return fail("attn_paged: q, out and scratch lie on 16-byte boundaries");
+    if (!(scale > 0.f) || !std::isfinite(scale)) return fail("attn_paged: the scale is not a positive number");
+    const size_t need = tm_cuda_attn_paged_scratch(T, c.B, max_q, H, c.KVH, c.dh);
+    if (scratch_bytes < need) return fail("attn_paged: %zu bytes of scratch, %zu are needed", scratch_bytes, need);
+    if (!on_library_device("attn_paged")) return false;
+    if (!T) return true;
+    return launch(c, kv_mask(window, sinks), kv->kv_half != 0, q, out, H, max_q ? max_q : T, scale, (cudaStream_t)stream);
+}
+
+bool tm_cuda_attn_window_dev(const float* q, const void* kc, const void* vc, float* scratch, size_t scratch_bytes, float* out, unsigned T,
+                             unsigned pos0, unsigned H, unsigned KVH, unsigned dh, unsigned ctx, unsigned window, unsigned sinks, float scale,
+                             int kv_half, void* stream) {
+    if (!q || !kc || !vc || !scratch || !out) return fail("attn_window: null pointer");
+    if (!KVH || !H || H % KVH || H / KVH > 128) return fail("attn_window: %u query heads for %u K/V heads (a multiple, at most 128 each)", H, KVH);
+    if (!dh || dh % 8 || dh > 128) return fail("attn_window: head dimension %u (multiples of 8 up to 128)", dh);
+    if (!ctx || ctx > 0x7fffffffu || pos0 > ctx || T > ctx - pos0) return fail("attn_window: positions %u to %llu of a cache of %u rows", pos0, (unsigned long long)pos0 + T, ctx);
+    if (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc | (uintptr_t)scratch | (uintptr_t)out) % 16) return fail("attn_window: q, the caches, scratch and out lie on 16-byte boundaries");
+    if (!(scale > 0.f) || !std::isfinite(scale)) return fail("attn_window: the scale is not a positive number");
+    const size_t need = tm_cuda_attn_window_scratch(T, H, KVH, dh);
+    if (scratch_bytes < need) return fail("attn_window: %zu bytes of scratch, %zu are needed", scratch_bytes, need);
+    if (!on_library_device("attn_window")) return false;
+    if (!T) return true;
+    const KvBatch c{kc, vc, nullptr, nullptr, nullptr, 1, KVH, dh, ctx, 1, 1, T, ctx, pos0 + T, -1};
+    return launch(c, kv_mask(window, sinks), kv_half != 0, q, out, H, T, scale, (cudaStream_t)stream);
+}
+
+}  // extern "C"

@@ -7,6 +7,7 @@
 // 2064-2079, 2141-2164). The token lane lives in token_lane.cu.
 #include "cuda_shim.h"
 #include "common.cuh"
+#include "kv_pages.cuh"
 #include "state.h"
 #include "gemm.h"
 
@@ -98,7 +99,7 @@ bool ensure_init(int device) {
     return true;
 }
 
-// Reads and clears the device status word the kernels set when a bounded wait ran out.
+// Reads and clears the device status word that kernels set when a bounded wait ran out or a batch's arrays name what is not there.
 bool harvest_status(const char* where) {
     State& s = state();
     const int h = *s.status_host;                        // the caller has just synchronised with the kernels
@@ -106,6 +107,7 @@ bool harvest_status(const char* where) {
         *s.status_host = 0;
         // lower this rank's sticky abort word, so that the next token's waits are real waits again
         if (s.peer.arena) cudaMemsetAsync((int*)s.peer.arena + kAbortWord, 0, sizeof(int), s.stream);
+        if (h == kStatusBatch) return fail("%s: a page, a length or a range of rows of a batch was out of range", where);
         return fail("%s: a kernel gave up on a bounded wait (status %d)", where, h);
     }
     return true;

@@ -1,0 +1,106 @@
+// kv_pages.cuh — what the kernels over a batch of sequences share: where a sequence's new tokens, positions and cache rows are,
+// and which keys a position sees. A contiguous cache [KVH][ctx][dh] is the same thing with one sequence and one page of ctx rows.
+#pragma once
+
+#include <stddef.h>
+#include <stdint.h>
+
+#ifdef __CUDACC__
+#include <cuda_runtime.h>
+#define TM_HD __host__ __device__ __forceinline__
+#else
+#define TM_HD inline                       // the index arithmetic is plain C++: a host test runs it against bad arrays
+#endif
+
+struct tm_cuda_kv_pages;
+
+namespace tmc {
+
+// A kernel argument. Every index that comes from device memory (table, q_begin, kv_len) is checked by the kernel that follows it:
+// what is out of range is not read, makes the results that depend on it NaN and sets the status word to kStatusBatch.
+struct KvBatch {
+    const void* k;
+    const void* v;
+    const int* table;           // nullptr: one sequence on one page, `total` positions, all T tokens new
+    const int* q_begin;
+    const int* kv_len;
+    uint32_t B, KVH, dh, page, npages, table_ld, T;
+    uint32_t cap;               // positions that a sequence's row of the table can name
+    uint32_t total;             // without a table: positions in the cache
+    int page_shift;             // log2(page), or -1
+};
+constexpr int kStatusBatch = 2;
+
+struct KvSeq {
+    uint32_t q0, n;             // its rows of q and out; none where q_begin does not give a range of them
+    int first;                  // position of the first new token (negative: more new tokens than positions)
+    uint32_t len;               // positions in the cache, the new tokens among them
+    bool lost, bad;             // no range of rows; no valid length (the rows are there, their results are NaN)
+};
+TM_HD KvSeq kv_seq(const KvBatch& c, uint32_t b) {
+    KvSeq s;
+    if (!c.table) {
+        s.q0 = 0; s.n = c.T; s.len = c.total; s.lost = s.bad = false;
+    } else {
+        const int a = c.q_begin[b], e = c.q_begin[b + 1], len = c.kv_len[b];
+        s.lost = a < 0 || e < a || (uint32_t)e > c.T;
+        s.q0 = s.lost ? 0u : (uint32_t)a;
+        s.n = s.lost ? 0u : (uint32_t)(e - a);
+        s.bad = len < 0 || (uint32_t)len > c.cap;
+        s.len = s.bad ? 0u : (uint32_t)len;
+    }
+    s.first = (int)s.len - (int)s.n;
+    return s;
+}
+// Element offset of row `pos` (< cap) of K/V head 0; row r of head h of the same page lies h * page * dh elements further. false: no such page.
+TM_HD bool kv_row(const KvBatch& c, uint32_t b, uint32_t pos, size_t* at) {
+    if (!c.table) { *at = (size_t)pos * c.dh; return true; }
+    uint32_t slot, row;
+    if (c.page_shift >= 0) { slot = pos >> c.page_shift; row = pos & (c.page - 1u); }
+    else { slot = pos / c.page; row = pos - slot * c.page; }
+    const uint32_t pg = (uint32_t)c.table[(size_t)b * c.table_ld + slot];
+    const bool ok = pg < c.npages;
+    *at = ((size_t)(ok ? pg : 0u) * c.KVH * c.page + row) * c.dh;
+    return ok;
+}
+
+#ifdef __CUDACC__
+__device__ __forceinline__ void note_bad_batch(int* status) {
+    if (status) *(volatile int*)status = kStatusBatch;
+}
+// The sequence that token t belongs to, found by a whole warp: as many q_begin[1..B] as are at most t. B: none.
+__device__ __forceinline__ uint32_t kv_find_seq(const KvBatch& c, uint32_t t) {
+    if (!c.table) return 0;
+    uint32_t before = 0;
+    for (uint32_t i = threadIdx.x & 31u; i < c.B; i += 32) before += c.q_begin[i + 1] <= (int)t;
+    return __reduce_add_sync(0xffffffffu, before);
+}
+#endif
+
+// Key j is seen from position p if it is not behind it and, with a window, less than `window` back or one of the first `sinks`.
+// window 0: no window. Neither is more than 2^31 - 1 (kv_mask).
+struct KvMask { uint32_t window, sinks; };
+inline KvMask kv_mask(unsigned window, unsigned sinks) { return KvMask{window > 0x7fffffffu ? 0u : window, sinks > 0x7fffffffu ? 0x7fffffffu : sinks}; }
+TM_HD bool kv_sees(const KvMask& m, int p, int j) {
+    return j <= p && (!m.window || (int)m.window > p - j || j < (int)m.sinks);
+}
+// The keys that positions [p0, p1] see between them: [0, a) and [b, e), a <= b.
+struct KvSpan { uint32_t a, b, e; };
+TM_HD KvSpan kv_span(const KvMask& m, int p0, int p1) {
+    KvSpan s;
+    s.e = p1 < 0 ? 0u : (uint32_t)p1 + 1u;
+    s.b = !m.window || p0 < (int)m.window ? 0u : (uint32_t)p0 - m.window + 1u;
+    s.a = !m.window ? 0u : m.sinks < s.b ? m.sinks : s.b;
+    return s;
+}
+
+// Partial results of a range of keys, for the merge of several: scores are kept in powers of two, and weights are 2^(s - m + kUp),
+// so that the halves into which a weight is split for the tensor cores stay in fp16's normal range down to 2^-28 of the largest.
+constexpr float kUp = 14.f;
+constexpr float kLog2e = 1.4426950408889634f;
+
+// host side (attn_pages.cu): the checks that every entry over such a batch makes; that the library is up on the current device
+bool kv_batch_from(KvBatch* c, const tm_cuda_kv_pages* kv, unsigned T, unsigned H, const char* who);
+bool on_library_device(const char* who);
+
+}  // namespace tmc

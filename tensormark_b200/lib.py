@@ -15,6 +15,19 @@ LIB_PATH = os.path.join(HERE, "libtm_cuda.so")
 _vp, _u, _sz, _u64 = C.c_void_p, C.c_uint, C.c_size_t, C.c_uint64
 _f32p = C.POINTER(C.c_float)
 
+
+class KvPages(C.Structure):
+    """tm_cuda_kv_pages: a batch of sequences and the paged cache that they are in. Pointers are device addresses."""
+    _fields_ = [("k", _vp), ("v", _vp), ("table", _vp), ("q_begin", _vp), ("kv_len", _vp), ("B", _u), ("KVH", _u), ("dh", _u),
+                ("page", _u), ("npages", _u), ("table_ld", _u), ("kv_half", C.c_int)]
+
+
+class LogitRules(C.Structure):
+    """tm_cuda_logit_rules: what a batch of requests asks of its logits. Pointers are device addresses; None leaves a rule out."""
+    _fields_ = [("tokens", _vp), ("n_tokens", _vp), ("n_prompt", _vp), ("repeat", _vp), ("presence", _vp), ("frequency", _vp),
+                ("bias_ids", _vp), ("bias", _vp), ("n_bias", _vp), ("mask", _vp), ("tokens_ld", _u), ("bias_ld", _u), ("mask_ld", _u)]
+
+
 # name -> (restype, argtypes); one line per entry of include/cuda_shim.h
 SIGNATURES = {
     "tm_cuda_init": (C.c_bool, [C.c_int]),
@@ -45,6 +58,12 @@ SIGNATURES = {
     "tm_cuda_attn_decode_scratch": (_sz, [_u, _u, _u, _u, _u]),
     "tm_cuda_attn_decode_dev": (C.c_bool, [_vp, _vp, _vp, _vp, _sz, _vp, _u, _u, _u, _u, _u, C.c_float, C.c_int, _vp]),
     "tm_cuda_attn_decode_static_dev": (C.c_bool, [_vp, _vp, _vp, _vp, _u, _u, _u, _u, _u, C.c_float, C.c_int, _vp]),
+    "tm_cuda_kv_append_paged_dev": (C.c_bool, [C.POINTER(KvPages), _vp, _vp, _u, _u, _vp, _u, _vp]),
+    "tm_cuda_attn_paged_scratch": (_sz, [_u, _u, _u, _u, _u, _u]),
+    "tm_cuda_attn_paged_dev": (C.c_bool, [C.POINTER(KvPages), _vp, _vp, _sz, _vp, _u, _u, _u, _u, _u, C.c_float, _vp]),
+    "tm_cuda_attn_window_scratch": (_sz, [_u, _u, _u, _u]),
+    "tm_cuda_attn_window_dev": (C.c_bool, [_vp, _vp, _vp, _vp, _sz, _vp, _u, _u, _u, _u, _u, _u, _u, _u, C.c_float, C.c_int, _vp]),
+    "tm_cuda_logits_rules_dev": (C.c_bool, [_vp, _sz, _vp, _sz, _u, _u, C.POINTER(LogitRules), _vp]),
     "tm_cuda_tok_begin": (C.c_bool, []),
     "tm_cuda_tok_flush": (C.c_bool, []),
     "tm_cuda_tok_end": (C.c_bool, [C.c_int, _vp, _u]),

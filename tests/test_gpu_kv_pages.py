@@ -1,0 +1,378 @@
+"""A batch of sequences over a paged K/V cache: append, attention of new tokens (one or many), windows and sinks, against plain
+implementations in 64 bits."""
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from tensormark_b200 import lib
+from tests.gpu_util import ptr, stream_ptr
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+class Batch:
+    """Random pages, lengths and queries; the pages that a sequence does not own hold NaN."""
+
+    def __init__(self, torch, new, total, H, KVH, dh, page, half, seed=0, extra_rows=0):
+        rng = np.random.default_rng(seed)
+        self.torch, self.new, self.total, self.H, self.KVH, self.dh, self.page, self.half = torch, new, list(total), H, KVH, dh, page, half
+        self.B, self.T = len(new), sum(new) + extra_rows
+        need = [-(-t // page) for t in total]
+        self.npages, self.ld = sum(need) + 2, max(need + [0]) + 1
+        order = rng.permutation(self.npages).astype(np.int32)
+        self.table = np.full((self.B, self.ld), -1, np.int32)
+        at = 0
+        for b, n in enumerate(need):
+            self.table[b, :n] = order[at:at + n]
+            at += n
+        kind = np.float16 if half else np.float32
+        self.k = rng.standard_normal((self.npages, KVH, page, dh)).astype(kind)
+        self.v = rng.standard_normal((self.npages, KVH, page, dh)).astype(kind)
+        for a in (self.k, self.v):
+            a[order[at:]] = np.nan
+            for b, t in enumerate(total):                                  # rows behind the last position, too
+                if t % page:
+                    a[self.table[b, t // page], :, t % page:] = np.nan
+        self.begin = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+        self.q = (rng.standard_normal((self.T, H * dh)) * 2).astype(np.float32)
+        self.upload()
+
+    def upload(self):
+        t = self.torch
+        up = lambda a: t.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+        self.d = {n: up(getattr(self, n)) for n in ("k", "v", "table", "q")}
+        self.d["q_begin"], self.d["kv_len"] = up(self.begin), up(np.asarray(self.total, np.int32))
+        self.desc = lib.KvPages(B=self.B, KVH=self.KVH, dh=self.dh, page=self.page, npages=self.npages, table_ld=self.ld, kv_half=int(self.half),
+                                **{n: self.d[n].data_ptr() for n in ("k", "v", "table", "q_begin", "kv_len")})
+
+    def rows(self, b):
+        j = np.arange(self.total[b])
+        pg = self.table[b, j // self.page]
+        return self.k[pg, :, j % self.page], self.v[pg, :, j % self.page]          # [len, KVH, dh]
+
+    def attend(self, cuda, window=0, sinks=0, max_q=None, scale=None, stream=None, want_ok=True):
+        t = self.torch
+        scale = 1 / np.sqrt(self.dh) if scale is None else scale
+        max_q = max(self.new) if max_q is None else max_q
+        need = cuda.tm_cuda_attn_paged_scratch(self.T, self.B, max_q, self.H, self.KVH, self.dh)
+        scratch = t.full((need // 4 + 1,), float("nan"), device="cuda")
+        out = t.full((self.T, self.H * self.dh), 7.0, device="cuda")
+        lib.check(cuda.tm_cuda_attn_paged_dev(C.byref(self.desc), ptr(self.d["q"]), ptr(scratch), need, ptr(out), self.T, max_q, self.H, window, sinks,
+                                              scale, stream_ptr(t)), "attn_paged")
+        t.cuda.synchronize()
+        assert cuda.tm_cuda_tok_flush() == want_ok, lib.last_error()
+        return out.cpu().numpy()
+
+    def check(self, cuda, window=0, sinks=0, **kw):
+        got = self.attend(cuda, window, sinks, **kw)
+        self.verify(got, window, sinks, kw.get("scale"))
+        assert np.all(got[self.begin[-1]:] == 7.0)                          # rows behind the last sequence
+        return got
+
+    def verify(self, got, window=0, sinks=0, scale=None, skip=()):
+        for b in set(range(self.B)) - set(skip):
+            q = self.q[self.begin[b]:self.begin[b + 1]].reshape(-1, self.H, self.dh)
+            k, v = self.rows(b)
+            want, tol = reference(q, k, v, self.total[b] - self.new[b], window, sinks, scale or 1 / np.sqrt(self.dh))
+            mine = got[self.begin[b]:self.begin[b + 1]].reshape(-1, self.H, self.dh)
+            assert np.array_equal(np.isnan(mine), np.isnan(want)), (b, "NaN in other places")
+            fine = np.isfinite(want)
+            assert np.array_equal(mine[~fine & ~np.isnan(want)], want[~fine & ~np.isnan(want)])
+            off = np.where(fine, np.abs(mine - np.where(fine, want, 0)), 0)
+            assert np.all(off[fine] <= tol[fine]), (b, float((off / np.where(tol > 0, tol, 1)).max()), float(off.max()))
+
+
+def reference(q, k, v, first, window, sinks, scale):
+    """q [n, H, dh], k and v [len, KVH, dh] -> out [n, H, dh] in 64 bits, and how far an fp32-grade kernel may be from it: a score is off by its
+    products' rounding (two halves of q: 2^-22, accumulation of dh products and their halves in any order: (dh + 8) roundings), at most
+    A (dh + 12) u with A the sum of their magnitudes; a weight by that (in powers of two: x log2 e, which the sums do not see, and a
+    rounding of the argument) + 2^-21; the sums of weights and products by as many roundings as there are additions in a chain, of
+    which a kernel that sums 16 keys at a time has len / 16 + 64. Numerator and denominator: twice."""
+    n, H, dh = q.shape
+    L, KVH = k.shape[0], k.shape[1]
+    out, tol = np.zeros((n, H, dh)), np.zeros((n, H, dh))
+    p, j = first + np.arange(n)[:, None], np.arange(L)[None]
+    seen = j <= p
+    if window:
+        seen &= (j > p - window) | (j < sinks)
+    with np.errstate(all="ignore"):
+        for h in range(H):
+            kk, vv = k[:, h // (H // KVH)].astype(np.float64), v[:, h // (H // KVH)].astype(np.float64)
+            for i in range(n):
+                vis = seen[i]
+                if not vis.any():
+                    continue
+                x, K, V = q[i, h].astype(np.float64), kk[vis], vv[vis]
+                s = K @ x * scale
+                A = np.abs(K) @ np.abs(x) * scale
+                w = np.exp(s - s.max())
+                w /= w.sum()
+                out[i, h] = w @ V
+                size = w @ np.abs(V)
+                tol[i, h] = 2 * size * ((A.max() if np.isfinite(A).all() else 0) * (dh + 13) * U + 2.0 ** -21 + (vis.sum() / 16 + 64) * U)
+    return out, tol
+
+
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("rep", [1, 2, 3, 4, 5, 8, 16])
+def test_single_tokens(cuda, torch_mod, rep, dh, half):
+    Batch(torch_mod, [1] * 5, [1, 16, 17, 333, 64], 2 * rep, 2, dh, 16, half, seed=rep).check(cuda)
+
+
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("rep,dh,page", [(4, 128, 16), (1, 64, 1), (3, 64, 24), (8, 128, 64), (7, 8, 5), (4, 80, 256), (20, 40, 16), (128, 64, 16), (5, 120, 48)])
+def test_chunks(cuda, torch_mod, rep, dh, page, half):
+    """Ragged chunks: one token to some hundred, chunks that are the whole sequence, sequences without new tokens, an empty cache."""
+    Batch(torch_mod, [1, 33, 0, 7, 130], [200, 33, 50, 8, 391], 2 * rep, 2, dh, page, half, seed=page).check(cuda)
+
+
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (16, 0), (63, 4), (64, 64), (100, 70), (130, 200), (5000, 4), (2 ** 31, 2 ** 32 - 1), (40, 2 ** 31)])
+def test_windows(cuda, torch_mod, window, sinks, half):
+    Batch(torch_mod, [1, 1, 70, 3], [1, 300, 333, 129], 8, 2, 64, 16, half, seed=window % 97).check(cuda, window, sinks)
+    Batch(torch_mod, [1, 2], [517, 90], 4, 1, 128, 7, half, seed=sinks % 89).check(cuda, window, sinks)
+
+
+@pytest.mark.parametrize("half", [True, False])
+def test_long_and_ragged(cuda, torch_mod, half):
+    Batch(torch_mod, [1] * 9, [4000, 1, 2, 700, 65, 64, 63, 5000, 128], 8, 2, 128, 16, half, seed=3).check(cuda)
+    Batch(torch_mod, [2, 300], [2500, 2000], 8, 2, 128, 32, half, seed=4).check(cuda)
+    Batch(torch_mod, [1] * 300, list(range(1, 301)), 4, 2, 64, 8, half, seed=5).check(cuda)
+
+
+@pytest.mark.parametrize("half", [True, False])
+def test_rows_that_see_nothing(cuda, torch_mod, half):
+    """More new tokens than positions: those before position 0 give zeros. Rows of q and out behind the last sequence stay."""
+    Batch(torch_mod, [3, 40, 5], [1, 0, 5], 4, 2, 64, 16, half, seed=1, extra_rows=4).check(cuda)
+
+
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("new,total", [([1, 1], [100, 40]), ([50, 100], [120, 100])])
+def test_nan_and_infinity_in_masked_places(cuda, torch_mod, new, total, half):
+    """Keys and values that only later tokens see, or that the window hides, hold NaN and infinity."""
+    b = Batch(torch_mod, new, total, 8, 2, 64, 16, half, seed=9)
+    for s, t in enumerate(total):
+        for pos, bad in ((t - 1, np.inf), (t - 2, np.nan), (20, -np.inf), (10, np.nan)):
+            pg = b.table[s, pos // 16]
+            b.v[pg, 1, pos % 16, ::3] = bad
+            b.k[pg, 0, pos % 16, 5] = np.nan
+    b.upload()
+    b.check(cuda, window=18, sinks=2)
+    b.check(cuda)
+
+
+@pytest.mark.parametrize("half", [True, False])
+def test_values_over_the_range(cuda, torch_mod, half):
+    """Large and small queries, keys near fp16's ends, weights that vanish: the scores decide, not the number format of the products."""
+    for gain in (1e-6, 1e-2, 30.0, 1e4):
+        b = Batch(torch_mod, [1, 40], [150, 200], 8, 2, 64, 16, half, seed=11)
+        b.q = (b.q * np.float32(gain)).astype(np.float32)
+        b.k = np.where(np.isnan(b.k), b.k, b.k * b.k.dtype.type(min(1.0, 10 / gain))).astype(b.k.dtype)
+        b.upload()
+        b.check(cuda)
+    b = Batch(torch_mod, [1, 40], [150, 200], 8, 2, 64, 16, half, seed=12)
+    b.k, b.v = (b.k * b.k.dtype.type(8000)).astype(b.k.dtype), (b.v * b.v.dtype.type(8000)).astype(b.v.dtype)
+    b.q[:, ::7] = 0
+    b.upload()
+    b.check(cuda, scale=1e-5)
+
+
+@pytest.mark.parametrize("rep,new", [(4, [1, 1, 1]), (4, [60, 1, 3])])
+def test_bad_arrays_are_reported(cuda, torch_mod, rep, new):
+    """A page, a length and a range of rows that are not there: NaN in the rows that need them, the others right, and an error."""
+    total = [max(t, n) for t, n in zip([40, 300, 77], new)]
+    make = lambda: Batch(torch_mod, new, total, 2 * rep, 2, 64, 16, True, seed=2)  # noqa: E731
+    for page in (-1, make().npages, 2 ** 31 - 1, -2 ** 31):
+        b = make()
+        b.table[1, 2] = page
+        b.upload()
+        got = b.attend(cuda, want_ok=False)
+        assert "out of range" in lib.last_error()
+        assert np.isnan(got[b.begin[1]:b.begin[2]]).all()
+        b.verify(got, skip=[1])
+    for length in (-1, make().ld * 16 + 1, 2 ** 31 - 1):
+        b = make()
+        b.total[1] = length
+        b.upload()
+        got = b.attend(cuda, want_ok=False)
+        assert np.isnan(got[b.begin[1]:b.begin[2]]).all()
+        b.verify(got, skip=[1])
+    for spoil, skip in ({2: b.T + 5, 3: b.T + 5}, [1, 2]), ({0: -3}, [0]), ({3: 2 ** 31 - 1}, [2]):
+        b = make()
+        good = b.begin.copy()
+        for i, v in spoil.items():
+            b.begin[i] = v
+        b.upload()
+        b.begin = good
+        got = b.attend(cuda, want_ok=False)
+        b.verify(got, skip=skip)
+        for i in skip:
+            assert np.all(got[good[i]:good[i + 1]] == 7.0)
+    b = make()
+    b.begin[2] = 0                                                         # not ascending: which rows are left is not said, only that it is noticed
+    b.upload()
+    b.attend(cuda, want_ok=False)
+
+
+def test_more_new_tokens_than_said(cuda, torch_mod):
+    """max_q is a promise: a sequence that breaks it gets NaN or its right rows, an error in the first case, and the others are right."""
+    b = Batch(torch_mod, [1, 40, 1], [100, 200, 30], 8, 2, 64, 16, True, seed=6)
+    want = b.check(cuda)
+    b.torch.cuda.synchronize()
+    need = cuda.tm_cuda_attn_paged_scratch(b.T, b.B, 1, b.H, b.KVH, b.dh)
+    scratch = torch_mod.empty(need // 4 + 1, device="cuda")
+    out = torch_mod.full((b.T, b.H * b.dh), 7.0, device="cuda")
+    assert cuda.tm_cuda_attn_paged_dev(C.byref(b.desc), ptr(b.d["q"]), ptr(scratch), need, ptr(out), b.T, 1, b.H, 0, 0, 0.125, stream_ptr(torch_mod))
+    torch_mod.cuda.synchronize()
+    assert not cuda.tm_cuda_tok_flush()
+    got = out.cpu().numpy()
+    assert np.isnan(got[1:41]).all() and np.array_equal(got[0], want[0]) and np.array_equal(got[41], want[41])
+
+
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("H,KVH,dh,T,pos0,ctx,window,sinks", [
+    (8, 2, 128, 1, 0, 1, 0, 0), (8, 2, 128, 1, 999, 1000, 100, 4), (32, 8, 64, 1, 4000, 4100, 1000, 4), (4, 1, 64, 200, 0, 200, 0, 0),
+    (6, 2, 80, 77, 130, 300, 50, 3), (8, 2, 128, 257, 300, 600, 64, 1), (16, 1, 128, 9, 77, 100, 0, 0), (5, 5, 64, 130, 1, 200, 200, 2),
+])
+def test_contiguous(cuda, torch_mod, H, KVH, dh, T, pos0, ctx, window, sinks, half):
+    t, rng = torch_mod, np.random.default_rng(pos0)
+    kind = np.float16 if half else np.float32
+    k, v = (rng.standard_normal((KVH, ctx, dh)).astype(kind) for _ in range(2))
+    k[:, pos0 + T:], v[:, pos0 + T:] = np.nan, np.nan
+    q = (rng.standard_normal((T, H * dh)) * 2).astype(np.float32)
+    kd, vd, qd = (t.from_numpy(a).cuda() for a in (k, v, q))
+    need = cuda.tm_cuda_attn_window_scratch(T, H, KVH, dh)
+    scratch, out = t.full((need // 4 + 1,), float("nan"), device="cuda"), t.full((T + 1, H * dh), 7.0, device="cuda")
+    lib.check(cuda.tm_cuda_attn_window_dev(ptr(qd), ptr(kd), ptr(vd), ptr(scratch), need, ptr(out), T, pos0, H, KVH, dh, ctx, window, sinks,
+                                           1 / np.sqrt(dh), int(half), stream_ptr(t)), "attn_window")
+    t.cuda.synchronize()
+    got = out.cpu().numpy()
+    assert np.all(got[T] == 7.0)
+    want, tol = reference(q.reshape(T, H, dh), k[:, :pos0 + T].transpose(1, 0, 2), v[:, :pos0 + T].transpose(1, 0, 2), pos0, window, sinks, 1 / np.sqrt(dh))
+    off = np.abs(got[:T].reshape(T, H, dh) - want)
+    assert np.all(off <= tol), float((off / tol).max())
+
+
+# ---- append --------------------------------------------------------------------------------------------------------------
+
+def append(cuda, b, rope, qkv, want_ok=True):
+    t = b.torch
+    q = t.full((b.T, b.H * b.dh), 7.0, device="cuda")
+    dq = t.from_numpy(qkv).cuda()
+    dr = t.from_numpy(rope).cuda() if rope is not None else None
+    lib.check(cuda.tm_cuda_kv_append_paged_dev(C.byref(b.desc), ptr(dq), ptr(q), b.T, b.H, ptr(dr) if rope is not None else None,
+                                               len(rope) if rope is not None else 0, stream_ptr(t)), "append")
+    t.cuda.synchronize()
+    assert cuda.tm_cuda_tok_flush() == want_ok
+    return q.cpu().numpy(), b.d["k"].cpu().numpy(), b.d["v"].cpu().numpy()
+
+
+def rope_table(n, dh, theta=10000.0):
+    a = np.arange(n)[:, None] * theta ** (-2.0 * np.arange(dh // 2) / dh)
+    return np.ascontiguousarray(np.stack((np.cos(a), np.sin(a)), -1).astype(np.float32))
+
+
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("H,KVH,dh,page,turned", [(8, 2, 128, 16, True), (4, 4, 64, 1, True), (6, 2, 80, 24, True), (5, 5, 8, 64, True), (8, 2, 64, 7, False)])
+def test_append(cuda, torch_mod, H, KVH, dh, page, turned, half):
+    new, total = [1, 70, 0, 3, 5], [100, 70, 9, 3, 4]                      # the last one: a token before position 0
+    b = Batch(torch_mod, new, total, H, KVH, dh, page, half, seed=dh, extra_rows=2)
+    rng = np.random.default_rng(1)
+    qkv = rng.standard_normal((b.T, (H + 2 * KVH) * dh)).astype(np.float32)
+    rope = rope_table(100, dh) if turned else None
+    q, k, v = append(cuda, b, rope, qkv)
+    wk, wv, wq = b.k.copy(), b.v.copy(), np.full((b.T, H, dh), 7.0)
+    touched = np.zeros(b.k.shape, bool)
+    tol = np.zeros((b.T, H, dh))
+    ktol = np.zeros(b.k.shape)
+    half_step = 2.0 ** -11 if half else 0.0
+    for s in range(b.B):
+        for i in range(new[s]):
+            p, t = total[s] - new[s] + i, b.begin[s] + i
+            if p < 0:
+                continue
+            x = qkv[t].reshape(-1, dh).astype(np.float64)
+            y, size = x.copy(), np.abs(x)
+            if turned:
+                c, sn = rope[p, :, 0].astype(np.float64), rope[p, :, 1].astype(np.float64)
+                lo, hi = x[:, :dh // 2], x[:, dh // 2:]
+                y = np.concatenate((lo * c - hi * sn, lo * sn + hi * c), 1)
+                size = np.concatenate((np.abs(lo * c) + np.abs(hi * sn), np.abs(lo * sn) + np.abs(hi * c)), 1)
+            wq[t], tol[t] = y[:H], 2 * U * size[:H]                        # a product's rounding and the sum's
+            pg, r = b.table[s, p // page], p % page
+            touched[pg, :, r] = True
+            wk[pg, :, r], wv[pg, :, r] = y[H:H + KVH], x[H + KVH:].astype(b.v.dtype)
+            ktol[pg, :, r] = 2 * U * size[H:H + KVH] + half_step * (np.abs(y[H:H + KVH]) * (1 + 2 * U)) * 2 + 2.0 ** -24 * half
+    assert np.all(np.abs(q.reshape(wq.shape) - wq) <= tol)
+    assert np.array_equal(v, wv, equal_nan=True)
+    assert np.array_equal(k[~touched], b.k[~touched], equal_nan=True)
+    assert np.all(np.abs(k[touched].astype(np.float64) - wk[touched]) <= ktol[touched])
+
+
+def test_append_checks_its_arrays(cuda, torch_mod):
+    H, KVH, dh, page = 4, 2, 64, 16
+    qkv = np.ones((4, (H + 2 * KVH) * dh), np.float32)
+    for spoil in ("page", "length", "range", "rope"):
+        b = Batch(torch_mod, [1, 2, 1], [40, 50, 20], H, KVH, dh, page, True, seed=3)
+        rope = rope_table(49 if spoil == "rope" else 64, dh)
+        if spoil == "page":
+            b.table[1, 3] = b.npages                                       # positions 48 and 49
+        if spoil == "length":
+            b.total = [40, b.ld * page + 1, 20]
+        if spoil == "range":
+            b.begin = np.array([0, 1, -1, 4], np.int32)
+        b.upload()
+        q, k, v = append(cuda, b, rope, qkv, want_ok=False)
+        changed = ~((v == b.v) | (np.isnan(v) & np.isnan(b.v)))
+        allowed = np.zeros_like(changed)
+        for s, p in ((0, 39), (2, 19)) + (((1, 48),) if spoil == "rope" else ()):
+            if spoil == "range" and s == 2:
+                continue
+            allowed[b.table[s, p // page], :, p % page] = True
+        assert not (changed & ~allowed).any(), spoil
+        assert changed[b.table[0, 2], :, 7].any() or spoil == "range"
+
+
+def test_append_then_attend_captured(cuda, torch_mod):
+    """A graph of append and attention, captured once, replayed for token after token with lengths that grow on the device."""
+    t = torch_mod
+    H, KVH, dh, page, steps = 8, 2, 64, 16, 20
+    start = [30, 1, 47]
+    b = Batch(t, [1, 1, 1], [s + steps for s in start], H, KVH, dh, page, True, seed=8)
+    rng = np.random.default_rng(5)
+    qkv = rng.standard_normal((steps, 3, (H + 2 * KVH) * dh)).astype(np.float32)
+    rope = rope_table(128, dh)
+    dr, dqkv, src = t.from_numpy(rope).cuda(), t.zeros(3, (H + 2 * KVH) * dh, device="cuda"), t.from_numpy(qkv).cuda()
+    q, out = t.zeros(3, H * dh, device="cuda"), t.zeros(3, H * dh, device="cuda")
+    need = cuda.tm_cuda_attn_paged_scratch(3, 3, 1, H, KVH, dh)
+    scratch = t.empty(need // 4 + 1, device="cuda")
+    side = t.cuda.Stream()
+    side.wait_stream(t.cuda.current_stream())
+
+    def step(s):
+        lib.check(cuda.tm_cuda_kv_append_paged_dev(C.byref(b.desc), ptr(dqkv), ptr(q), 3, H, ptr(dr), 128, s), "append")
+        lib.check(cuda.tm_cuda_attn_paged_dev(C.byref(b.desc), ptr(q), ptr(scratch), need, ptr(out), 3, 1, H, 25, 2, 0.125, s), "attend")
+
+    with t.cuda.stream(side):
+        b.d["kv_len"].copy_(t.tensor(start, dtype=t.int32))
+        step(stream_ptr(t))
+    side.synchronize()
+    graph = t.cuda.CUDAGraph()
+    with t.cuda.graph(graph):
+        step(stream_ptr(t))
+    for i in range(steps):
+        dqkv.copy_(src[i])
+        b.d["kv_len"].copy_(t.tensor([s + i + 1 for s in start], dtype=t.int32))
+        graph.replay()
+        t.cuda.synchronize()
+        b.k, b.v = b.d["k"].cpu().numpy(), b.d["v"].cpu().numpy()
+        b.total = [s + i + 1 for s in start]
+        got, qs = out.cpu().numpy(), q.cpu().numpy()
+        for s in range(3):
+            want, tol = reference(qs[s].reshape(1, H, dh), *b.rows(s), b.total[s] - 1, 25, 2, 0.125)
+            assert np.all(np.abs(got[s].reshape(1, H, dh) - want) <= tol)
