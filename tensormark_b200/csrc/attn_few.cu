@@ -1,0 +1,593 @@
+// attn_few.cu — attention of sequences that bring few query rows (a decode step, a handful of drafted tokens) over a paged cache.
+//
+// out = sum_j p_j v_j / sum_j p_j, p_j = 2^(s_j - m), s = scale log2(e) q k, with the running maximum m of one pass over the keys.
+//
+// Bound: HBM, every visible K and V row is read once for all the query rows of its head. The work of the whole batch - (sequence,
+// K/V head, tile of 64 keys), tiles in order - is one list of which every CTA takes an equal stretch, whatever the lengths are; a
+// CTA finishes the units that lie in its stretch and leaves a partial of the one or two that it shares, which a second kernel merges.
+//   * A warp takes 16 keys of every tile through a ring of its own (cp.async, one lane looks up one row's page), so nothing in the
+//     loop waits for another warp.
+//   * Both products run on mma.sync with the query rows as its 16 rows: the keys' and values' bytes are the traffic, so the padding
+//     costs nothing that counts. Results are to be as good as fp32's, so an fp32 operand is two fp16 parts (two tf32 parts against
+//     fp32 caches), high and low: error 2^-22. With at most 8 rows the parts are the two halves of the 16 rows: one product.
+//     q is scaled by a power of two per row, and weights by 2^14, which keeps the low parts in fp16's normal range.
+//   * The output is summed in fp32 registers, 16 keys at a time: a tensor core's own running sum is cut, not rounded, at every step.
+//   * A value that is masked for one row but not for another meets a weight of 0 in the product, which is NaN if the value is not
+//     finite. So a result that is not finite is computed again row by row, where masked keys are skipped.
+#include "attn_pages.h"
+#include "common.cuh"
+#include "per_device.h"
+
+#include <algorithm>
+#include <cuda_fp16.h>
+#include <math_constants.h>
+#include <type_traits>
+
+namespace tmc {
+namespace {
+
+constexpr uint32_t kWarps = 4, kTile = 64, kStep = 16;      // keys of a tile; of a warp's share of it
+
+__device__ __forceinline__ float pow2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t bytes) {   // bytes 0: zeros
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// x, y as fp16 pairs: the rounded values and what the rounding left
+__device__ __forceinline__ void parts(float x, float y, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = half2_bits(x - f.x, y - f.y);
+}
+__device__ __forceinline__ void parts(float x, uint32_t& hi, uint32_t& lo) {             // tf32: the low part is cut to 11 bits by the product
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+    lo = __float_as_uint(x - __uint_as_float(hi));
+}
+
+// ---- the list of work ------------------------------------------------------------------------------------------------
+struct Unit {                       // the keys of one sequence, tile by tile: [0, a) and [b, e) in tiles that start at multiples of kTile
+    KvSeq s;
+    uint32_t tiles, head_tiles, skip;        // tile t starts at key t * kTile, or (t + skip) * kTile from head_tiles on
+    uint32_t end;                   // keys from here on are behind every row's position
+    bool bad;                       // its rows are NaN
+};
+__device__ __forceinline__ uint32_t tile_key(const Unit& u, uint32_t t) { return (t < u.head_tiles ? t : t + u.skip) * kTile; }
+__device__ Unit unit_of(const AttnCall& a, uint32_t b) {
+    Unit u;
+    u.s = kv_seq(a.c, b);
+    u.bad = u.s.bad || u.s.n > a.max_q;
+    const uint32_t rows = u.s.n <= a.few ? u.s.n * a.rep : a.few + 1;       // no overflow
+    if (u.s.n == 0 || (rows > a.few && a.others)) { u.tiles = 0; return u; }
+    const KvSpan sp = kv_span(a.mask, u.s.first, (int)u.s.len - 1);
+    u.end = u.bad ? 0u : sp.e;
+    const uint32_t e = (u.end + kTile - 1) / kTile, lo = sp.b / kTile;
+    u.head_tiles = (sp.a + kTile - 1) / kTile;
+    u.skip = lo > u.head_tiles ? lo - u.head_tiles : 0u;
+    u.tiles = max(1u, e - min(e, u.skip));
+    return u;
+}
+
+struct Part { int b, h, last, first; };     // of CTA c: the unit in whose middle its stretch begins, the CTA that ends it, whether c is the first that begins in it
+
+template <typename T, int DHP, bool PAIR> struct Few {
+    static constexpr uint32_t Rows = PAIR ? 8 : 16;
+    static constexpr uint32_t RowBytes = DHP * sizeof(T), StageBytes = 2 * kStep * RowBytes;     // K and V of a warp's step
+    static constexpr uint32_t Stages = sizeof(T) == 4 ? (DHP == 128 ? (PAIR ? 3 : 2) : 4) : (PAIR ? 3 : 2) * (128 / DHP);
+    static constexpr uint32_t Ring = kWarps * Stages * StageBytes, Merge = kWarps * Rows * DHP * 4;
+    static constexpr uint32_t Smem = Ring + Merge;
+    static constexpr uint32_t PerSm = Smem <= 114688 ? 2 : 1;
+};
+
+// The rows of a unit over tiles [t0, t1) once more, key by key: to part and stat, or, where the unit is all there, to out.
+template <typename T>
+__device__ __noinline__ void rows_again(const AttnCall& a, const Unit& u, uint32_t b, uint32_t h, uint32_t t0, uint32_t t1, float* part, float2* stat) {
+    const uint32_t lane = threadIdx.x & 31u, dh = a.c.dh;
+    const T* kb = (const T*)a.c.k + (size_t)h * a.c.page * dh;
+    const T* vb = (const T*)a.c.v + (size_t)h * a.c.page * dh;
+    for (uint32_t r = threadIdx.x >> 5; r < u.s.n * a.rep; r += kWarps) {
+        const int p = u.s.first + (int)(r / a.rep);
+        const size_t row = ((size_t)(u.s.q0 + r / a.rep) * a.H + h * a.rep + r % a.rep) * dh;
+        float qr[4], acc[4] = {}, m = -CUDART_INF_F, l = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) qr[k] = lane + 32u * k < dh ? a.q[row + lane + 32u * k] * (a.scale * kLog2e) : 0.f;
+        for (uint32_t t = t0; t < t1; ++t) {
+            const uint32_t j0 = tile_key(u, t);
+            for (uint32_t j = j0; j < min(j0 + kTile, u.end); ++j) {
+                size_t at;
+                if (!kv_sees(a.mask, p, (int)j) || !kv_row(a.c, b, j, &at)) continue;
+                float x = 0.f;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (lane + 32u * k < dh) x = fmaf(qr[k], (float)kb[at + lane + 32u * k], x);
+#pragma unroll
+                for (int s = 16; s; s >>= 1) x += __shfl_xor_sync(0xffffffffu, x, s);
+                const float mn = fmaxf(m, x), corr = m == -CUDART_INF_F ? 0.f : exp2f(m - mn), w = x == -CUDART_INF_F ? 0.f : exp2f(x - mn + kUp);
+                l = fmaf(l, corr, w);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (lane + 32u * k < dh) acc[k] = fmaf(acc[k], corr, w * (float)vb[at + lane + 32u * k]);
+                m = mn;
+            }
+        }
+        float* to = stat ? part + (size_t)r * dh : a.out + row;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (lane + 32u * k < dh) to[lane + 32u * k] = stat ? acc[k] : l == 0.f ? 0.f : acc[k] / l;
+        if (stat && lane == 0) stat[r] = make_float2(m, l);
+    }
+}
+
+template <typename T, int DHP, bool PAIR>
+__global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_few_kernel(const __grid_constant__ AttnCall a, float* part, float2* stat, Part* meta) {
+    using F = Few<T, DHP, PAIR>;
+    constexpr bool kHalf = sizeof(T) == 2;
+    constexpr uint32_t RB = F::RowBytes, SB = F::StageBytes, S = F::Stages, ROWS = F::Rows, NB = DHP / 8, NR = PAIR ? 1 : 2;
+    constexpr uint32_t KS = DHP / 16;                       // 16 dims at a time, whatever the type
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ unsigned long long sums[kWarps];
+    __shared__ uint32_t at_b, at_h, at_t;
+    __shared__ float sm_m[kWarps][ROWS], sm_l[kWarps][ROWS];
+    __shared__ int sm_bad[2];
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g = lane >> 2, t4 = lane & 3u;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const uint32_t dh = a.c.dh, KVH = a.c.KVH;
+
+    // ---- this CTA's stretch of the list ----
+    unsigned long long x0, x1, total;
+    {
+        const uint32_t per = (a.c.B + blockDim.x - 1) / blockDim.x, b0 = min(a.c.B, tid * per), b1 = min(a.c.B, b0 + per);
+        unsigned long long mine = 0;
+        for (uint32_t b = b0; b < b1; ++b) {
+            const Unit u = unit_of(a, b);
+            if (u.s.lost && blockIdx.x == 0) note_bad_batch(a.status);
+            mine += (unsigned long long)u.tiles * KVH;
+        }
+        unsigned long long incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const unsigned long long y = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= (uint32_t)o) incl += y; }
+        if (lane == 31) sums[warp] = incl;
+        if (tid == 0) { at_b = a.c.B; at_h = at_t = 0; sm_bad[0] = sm_bad[1] = 0; }
+        __syncthreads();
+        total = 0;
+        unsigned long long before = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < kWarps; ++w) { if (w == warp) before = total; total += sums[w]; }
+        const unsigned long long per_cta = total / gridDim.x, rem = total % gridDim.x, c = blockIdx.x;
+        x0 = c * per_cta + min(c, rem); x1 = x0 + per_cta + (c < rem ? 1 : 0);
+        unsigned long long x = before + incl - mine;
+        if (x0 >= x && x0 < x + mine) {                     // the stretch begins in one of this thread's sequences
+            for (uint32_t b = b0; b < b1; ++b) {
+                const Unit u = unit_of(a, b);
+                const unsigned long long n = (unsigned long long)u.tiles * KVH;
+                if (x0 < x + n) {
+                    const uint32_t h = (uint32_t)((x0 - x) / u.tiles), t = (uint32_t)((x0 - x) % u.tiles);
+                    at_b = b; at_h = h; at_t = t;
+                    Part p{-1, 0, 0, 0};
+                    if (t && x1 > x0) {
+                        const unsigned long long start = x0 - t, end = start + u.tiles - 1, line = rem * (per_cta + 1);
+                        p.b = (int)b; p.h = (int)h;
+                        p.last = (int)(end < line ? end / (per_cta + 1) : rem + (end - line) / per_cta);
+                        const unsigned long long back = x0 - per_cta - (c - 1 < rem ? 1 : 0);         // where CTA c - 1 begins
+                        p.first = start >= back;
+                    }
+                    meta[blockIdx.x] = p;
+                    break;
+                }
+                x += n;
+            }
+        }
+        __syncthreads();
+        if (x1 == x0) {
+            if (tid == 0) meta[blockIdx.x] = Part{-1, 0, 0, 0};
+            return;
+        }
+    }
+
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * (S * SB);
+    float* const merge = reinterpret_cast<float*>(smem + F::Ring);
+    if (dh < DHP) {                                         // dims that no copy writes
+        for (uint32_t i = tid * 16; i < F::Ring; i += blockDim.x * 16) *reinterpret_cast<uint4*>(smem + i) = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+    }
+
+    // ---- the copies: a cursor of their own, Stages - 1 tiles ahead ----
+    uint32_t lb = at_b, lh = at_h, lt = at_t, left = (uint32_t)(x1 - x0), slot = 0;
+    uint32_t no_page = 0;                                   // bit of a stage: a page was not there
+    Unit lu = unit_of(a, lb);
+    auto request = [&]() {
+        if (left) {
+            const uint32_t j = tile_key(lu, lt) + warp * kStep + (lane & 15u);
+            size_t at = 0;
+            const bool in = j < lu.end;
+            bool ok = true;
+            if (in) ok = kv_row(a.c, lb, j, &at);
+            no_page = no_page & ~(1u << slot) | (__any_sync(0xffffffffu, !ok) ? 1u << slot : 0u);
+            at = (at + (size_t)lh * a.c.page * dh) * sizeof(T);
+            const uint32_t chunks = dh * (uint32_t)sizeof(T) / 16, lo = (uint32_t)at, hi = (uint32_t)(at >> 32);
+            const uint32_t there = __ballot_sync(0xffffffffu, in && ok);
+            constexpr uint32_t C = RB / 16, RP = 32 / C > 0 ? 32 / C : 1;            // chunks of a row; rows of a round
+            const uint32_t dst = ring + slot * SB;
+#pragma unroll
+            for (uint32_t i = 0; i < kStep / RP; ++i) {
+                const uint32_t r = i * RP + lane / C, ch = lane % C;
+                const size_t off = (size_t)__shfl_sync(0xffffffffu, lo, r) | (size_t)__shfl_sync(0xffffffffu, hi, r) << 32;
+                if (ch < chunks) {
+                    const uint32_t n = there >> r & 1u ? 16u : 0u;
+                    const uint32_t kx = kHalf ? r & 7u : (r & 3u) << 1 | (r >> 2 & 1u);
+                    copy16(dst + r * RB + ((ch ^ kx) << 4), (const uint8_t*)a.c.k + off + ch * 16, n);
+                    copy16(dst + kStep * RB + r * RB + ((ch ^ (r & 7u)) << 4), (const uint8_t*)a.c.v + off + ch * 16, n);
+                }
+            }
+            if (--left && ++lt == lu.tiles) {
+                lt = 0;
+                if (++lh == KVH) {
+                    lh = 0;
+                    lu.tiles = 0;
+                    while (lu.tiles == 0 && ++lb < a.c.B) lu = unit_of(a, lb);
+                    if (lb >= a.c.B) left = 0;              // the arrays are not what they were: nothing behind them is read
+                }
+            }
+        }
+        if (++slot == S) slot = 0;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (uint32_t i = 0; i + 1 < S; ++i) request();
+
+    // ---- the units of the stretch ----
+    uint32_t b = at_b, h = at_h, t = at_t, todo = (uint32_t)(x1 - x0), use = 0, turn = 0;
+    Unit u = unit_of(a, b);
+    for (;;) {
+        const uint32_t t0 = t, t1 = min(u.tiles, t + todo), rows = min(u.s.n * a.rep, ROWS);
+        int pos[NR];
+        float back[NR], m[NR], l[NR], o[NB][2 * NR];        // back: what undoes q's power of two
+        uint32_t qf[NR][KS][4];                             // fp16: the fragments, both parts; fp32: the values of a row
+        {
+            const float* qp[NR];
+#pragma unroll
+            for (uint32_t n = 0; n < NR; ++n) {
+                const uint32_t r = g + 8 * n, i = r / a.rep;
+                const bool is = r < rows;
+                pos[n] = is ? u.s.first + (int)i : -1;
+                qp[n] = is ? a.q + ((size_t)(u.s.q0 + i) * a.H + h * a.rep + r % a.rep) * dh : nullptr;
+                m[n] = -CUDART_INF_F; l[n] = 0.f; back[n] = 1.f;
+                float2 raw[2 * KS];
+#pragma unroll
+                for (uint32_t k = 0; k < 2 * KS; ++k) {
+                    const uint32_t d = k * 8 + 2 * t4;
+                    raw[k] = make_float2(0.f, 0.f);
+                    if (is && d < dh) raw[k] = *reinterpret_cast<const float2*>(qp[n] + d);
+                    raw[k].x *= a.scale * kLog2e; raw[k].y *= a.scale * kLog2e;
+                }
+                if constexpr (kHalf) {
+                    float top = 0.f;
+#pragma unroll
+                    for (uint32_t k = 0; k < 2 * KS; ++k) top = fmaxf(top, fmaxf(fabsf(raw[k].x), fabsf(raw[k].y)));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 120);      // the row's largest to [2^13, 2^14)
+                    const float up = __uint_as_float((uint32_t)(127 + 13 - e) << 23);
+                    back[n] = __uint_as_float((uint32_t)(127 - 13 + e) << 23);
+#pragma unroll
+                    for (uint32_t k = 0; k < 2 * KS; ++k) {
+                        uint32_t hi, lo;
+                        parts(raw[k].x * up, raw[k].y * up, hi, lo);
+                        if constexpr (PAIR) { qf[0][k / 2][2 * (k & 1)] = hi; qf[0][k / 2][2 * (k & 1) + 1] = lo; }
+                        else { qf[0][k / 2][2 * (k & 1) + n] = hi; qf[NR - 1][k / 2][2 * (k & 1) + n] = lo; }
+                    }
+                } else {
+#pragma unroll
+                    for (uint32_t k = 0; k < 2 * KS; ++k) { qf[n][k / 2][2 * (k & 1)] = __float_as_uint(raw[k].x); qf[n][k / 2][2 * (k & 1) + 1] = __float_as_uint(raw[k].y); }
+                }
+            }
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < NB; ++i)
+#pragma unroll
+            for (uint32_t k = 0; k < 2 * NR; ++k) o[i][k] = 0.f;
+        bool lost_page = false;
+
+        for (; t < t1; ++t) {
+            request();
+            asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
+            __syncwarp();
+            const uint32_t kat = ring + use * SB, vat = kat + kStep * RB, j0 = tile_key(u, t) + warp * kStep;
+            if (no_page >> use & 1u) lost_page = true;
+            if (j0 < u.end) {
+                float s[2][4] = {};
+                if constexpr (kHalf) {
+                    const uint32_t key = (lane >> 4) * 8 + (lane & 7u), row = kat + key * RB, c0 = lane >> 3 & 1u;
+#pragma unroll
+                    for (uint32_t k = 0; k < KS; ++k) {
+                        uint32_t f[4];
+                        ldsm4(f, row + (((2 * k + c0) ^ (key & 7u)) << 4));
+#pragma unroll
+                        for (uint32_t n = 0; n < NR; ++n) { mma_f16(s[0], qf[n][k], f[0], f[1]); mma_f16(s[1], qf[n][k], f[2], f[3]); }
+                    }
+                } else {
+#pragma unroll
+                    for (uint32_t k = 0; k < 2 * KS; ++k) {
+                        uint32_t ah[4], al[4];              // PAIR: ah holds both parts
+#pragma unroll
+                        for (uint32_t n = 0; n < NR; ++n) {
+                            uint32_t h0, l0, h1, l1;
+                            parts(__uint_as_float(qf[n][k / 2][2 * (k & 1)]), h0, l0);
+                            parts(__uint_as_float(qf[n][k / 2][2 * (k & 1) + 1]), h1, l1);
+                            if constexpr (PAIR) { ah[0] = h0; ah[1] = l0; ah[2] = h1; ah[3] = l1; }
+                            else { ah[n] = h0; al[n] = l0; ah[2 + n] = h1; al[2 + n] = l1; }
+                        }
+#pragma unroll
+                        for (uint32_t nb = 0; nb < 2; ++nb) {
+                            const uint32_t key = nb * 8 + g, kx = (key & 3u) << 1 | (key >> 2 & 1u);
+                            float2 f;
+                            asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(f.x), "=f"(f.y) : "r"(kat + key * RB + (((2 * k + (t4 >> 1)) ^ kx) << 4) + (t4 & 1u) * 8));
+                            uint32_t h0, l0, h1, l1;
+                            parts(f.x, h0, l0); parts(f.y, h1, l1);
+                            mma_tf32(s[nb], ah, h0, h1);
+                            mma_tf32(s[nb], ah, l0, l1);
+                            if constexpr (!PAIR) mma_tf32(s[nb], al, h0, h1);
+                        }
+                    }
+                }
+                const bool whole = (int)j0 + (int)kStep - 1 <= u.s.first &&
+                                   (!a.mask.window || j0 + a.mask.window >= u.s.len || j0 + kStep <= a.mask.sinks);
+                float corr[NR];
+                uint32_t ph[NR][4];                         // the weights as the second product's rows: PAIR: [0] both parts; else high, low
+#pragma unroll
+                for (uint32_t n = 0; n < NR; ++n) {
+                    float x[4];
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i) {
+                        if constexpr (PAIR) x[i] = (s[i >> 1][i & 1] + s[i >> 1][2 + (i & 1)]) * back[0];
+                        else x[i] = s[i >> 1][2 * n + (i & 1)] * back[n];
+                    }
+                    if (!whole) {
+#pragma unroll
+                        for (uint32_t i = 0; i < 4; ++i)
+                            if (!kv_sees(a.mask, pos[n], (int)(j0 + (i >> 1) * 8 + 2 * t4 + (i & 1)))) x[i] = -CUDART_INF_F;
+                    }
+                    float mn = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                    mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 1));
+                    mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 2));
+                    mn = fmaxf(mn, m[n]);
+                    const float base = mn == -CUDART_INF_F ? 0.f : mn;
+                    corr[n] = pow2(m[n] - base);
+                    m[n] = mn;
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i) x[i] = pow2(x[i] - base + kUp);
+                    l[n] = fmaf(l[n], corr[n], (x[0] + x[1]) + (x[2] + x[3]));
+                    if constexpr (kHalf) {
+                        if constexpr (PAIR) { parts(x[0], x[1], ph[0][0], ph[0][1]); parts(x[2], x[3], ph[0][2], ph[0][3]); }
+                        else { parts(x[0], x[1], ph[0][n], ph[NR - 1][n]); parts(x[2], x[3], ph[0][2 + n], ph[NR - 1][2 + n]); }
+                    } else {
+#pragma unroll
+                        for (uint32_t i = 0; i < 4; ++i) ph[n][i] = __float_as_uint(x[i]);
+                    }
+                }
+                if constexpr (kHalf) {
+                    const uint32_t key = (lane >> 3 & 1u) * 8 + (lane & 7u), row = vat + key * RB, c0 = lane >> 4;
+#pragma unroll
+                    for (uint32_t i = 0; i < NB / 2; ++i) {
+                        uint32_t f[4];
+                        ldsm4_t(f, row + (((2 * i + c0) ^ (key & 7u)) << 4));
+#pragma unroll
+                        for (uint32_t k = 0; k < 2; ++k) {
+                            float d[4] = {};
+#pragma unroll
+                            for (uint32_t n = 0; n < NR; ++n) mma_f16(d, ph[n], f[2 * k], f[2 * k + 1]);
+                            float (&to)[2 * NR] = o[2 * i + k];
+                            if constexpr (PAIR) { to[0] = fmaf(to[0], corr[0], d[0] + d[2]); to[1] = fmaf(to[1], corr[0], d[1] + d[3]); }
+                            else {
+#pragma unroll
+                                for (uint32_t e = 0; e < 4; ++e) to[e] = fmaf(to[e], corr[NR == 1 ? 0 : e >> 1], d[e]);
+                            }
+                        }
+                    }
+                } else {
+                    uint32_t ah[2][4], al[2][4];            // key 2 t of a block of 8 is row t of the product's operand, key 2 t + 1 row t + 4
+#pragma unroll
+                    for (uint32_t nb = 0; nb < 2; ++nb)
+#pragma unroll
+                        for (uint32_t n = 0; n < NR; ++n) {
+                            uint32_t h0, l0, h1, l1;
+                            parts(__uint_as_float(ph[n][2 * nb]), h0, l0);
+                            parts(__uint_as_float(ph[n][2 * nb + 1]), h1, l1);
+                            if constexpr (PAIR) { ah[nb][0] = h0; ah[nb][1] = l0; ah[nb][2] = h1; ah[nb][3] = l1; }
+                            else { ah[nb][n] = h0; al[nb][n] = l0; ah[nb][2 + n] = h1; al[nb][2 + n] = l1; }
+                        }
+#pragma unroll
+                    for (uint32_t i = 0; i < NB; ++i) {
+                        float d[4] = {};
+#pragma unroll
+                        for (uint32_t nb = 0; nb < 2; ++nb) {
+                            uint32_t vh[2], vl[2];
+#pragma unroll
+                            for (uint32_t k = 0; k < 2; ++k) {
+                                const uint32_t key = nb * 8 + 2 * t4 + k;
+                                float f;
+                                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(vat + key * RB + (((2 * i + (g >> 2)) ^ (key & 7u)) << 4) + (g & 3u) * 4));
+                                parts(f, vh[k], vl[k]);
+                            }
+                            mma_tf32(d, ah[nb], vh[0], vh[1]);
+                            mma_tf32(d, ah[nb], vl[0], vl[1]);
+                            if constexpr (!PAIR) mma_tf32(d, al[nb], vh[0], vh[1]);
+                        }
+                        float (&to)[2 * NR] = o[i];
+                        if constexpr (PAIR) { to[0] = fmaf(to[0], corr[0], d[0] + d[2]); to[1] = fmaf(to[1], corr[0], d[1] + d[3]); }
+                        else {
+#pragma unroll
+                            for (uint32_t e = 0; e < 4; ++e) to[e] = fmaf(to[e], corr[NR == 1 ? 0 : e >> 1], d[e]);
+                        }
+                    }
+                }
+            }
+            __syncwarp();                                   // the stage is free for the next request
+            if (++use == S) use = 0;
+        }
+
+        // ---- the warps' results together ----
+#pragma unroll
+        for (uint32_t n = 0; n < NR; ++n) {
+            l[n] += __shfl_xor_sync(0xffffffffu, l[n], 1);
+            l[n] += __shfl_xor_sync(0xffffffffu, l[n], 2);
+            if (t4 == 0) { sm_m[warp][g + 8 * n] = m[n]; sm_l[warp][g + 8 * n] = l[n]; }
+#pragma unroll
+            for (uint32_t i = 0; i < NB; ++i)
+                *reinterpret_cast<float2*>(merge + ((size_t)warp * ROWS + g + 8 * n) * DHP + i * 8 + 2 * t4) = make_float2(o[i][2 * n], o[i][2 * n + 1]);
+        }
+        if ((lost_page || u.bad) && lane == 0) sm_bad[turn] = 1;
+        __syncthreads();
+        const bool bad = sm_bad[turn], all = t0 == 0 && t1 == u.tiles;
+        const size_t slot = 2 * (size_t)blockIdx.x + (t0 == 0);            // of a unit that began before: 0; that goes on behind: 1
+        float* const po = part + slot * ROWS * dh;
+        float2* const ps = stat + slot * ROWS;
+        bool again = false;
+        if (tid < dh) {
+            for (uint32_t r = 0; r < rows; ++r) {
+                float M = -CUDART_INF_F, x = 0.f, L = 0.f;
+#pragma unroll
+                for (uint32_t w = 0; w < kWarps; ++w) M = fmaxf(M, sm_m[w][r]);
+#pragma unroll
+                for (uint32_t w = 0; w < kWarps; ++w) {
+                    const float f = sm_m[w][r] == -CUDART_INF_F ? 0.f : pow2(sm_m[w][r] - M);
+                    x = fmaf(f, merge[((size_t)w * ROWS + r) * DHP + tid], x);
+                    L = fmaf(f, sm_l[w][r], L);
+                }
+                again = again || !(fabsf(x) < CUDART_INF_F) || !(fabsf(L) < CUDART_INF_F);
+                if (bad) L = CUDART_NAN_F;
+                if (all) {
+                    a.out[((size_t)(u.s.q0 + r / a.rep) * a.H + h * a.rep + r % a.rep) * dh + tid] = L == 0.f ? 0.f : x / L;
+                } else {
+                    po[(size_t)r * dh + tid] = x;
+                    if (tid == 0) ps[r] = make_float2(M, L);
+                }
+            }
+            if (bad)                                        // more rows than were promised
+                for (uint32_t r = rows; r < u.s.n * a.rep; ++r) a.out[((size_t)(u.s.q0 + r / a.rep) * a.H + h * a.rep + r % a.rep) * dh + tid] = CUDART_NAN_F;
+        }
+        if (bad && tid == 0) note_bad_batch(a.status);
+        if (tid == 0) sm_bad[turn ^ 1u] = 0;
+        if (__syncthreads_or(again && !bad)) rows_again<T>(a, u, b, h, t0, t1, po, all ? nullptr : ps);
+        turn ^= 1u;
+        todo -= t1 - t0;
+        if (!todo) return;
+        t = 0;
+        if (++h == KVH) {
+            h = 0;
+            u.tiles = 0;
+            while (u.tiles == 0 && ++b < a.c.B) u = unit_of(a, b);
+            if (b >= a.c.B) return;
+        }
+    }
+}
+
+// One CTA per stretch that begins inside a unit, of which the first of a unit merges all of its parts: the last of the CTA before, and the
+// first of its own and of those behind it. Rows over blockIdx.y; four threads per dim take every fourth part.
+constexpr uint32_t kMergeGroups = 4;
+__global__ void __launch_bounds__(kMergeGroups * 128) attn_few_merge_kernel(const __grid_constant__ AttnCall a, const float* part, const float2* stat, const Part* meta, uint32_t slot_rows) {
+    __shared__ float so[kMergeGroups][128];
+    __shared__ float2 sml[kMergeGroups];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const uint32_t c = blockIdx.x + 1, r = blockIdx.y, d = threadIdx.x, grp = threadIdx.y, dh = a.c.dh;
+    const Part p = meta[c];
+    if (p.b < 0 || !p.first) return;
+    const KvSeq s = kv_seq(a.c, (uint32_t)p.b);
+    if (r >= s.n * a.rep) return;
+    const uint32_t parts = (uint32_t)p.last - c + 2;
+    float M = -CUDART_INF_F, L = 0.f, o = 0.f;
+    for (uint32_t i = grp; i < parts; i += kMergeGroups) {
+        const size_t row = (size_t)(2 * (c + i) - (i ? 2 : 1)) * slot_rows + r;        // i = 0: slot 1 of CTA c - 1; else slot 0 of CTA c + i - 1
+        const float2 ml = stat[row];
+        const float x = d < dh ? part[row * dh + d] : 0.f, mn = fmaxf(M, ml.x);
+        const float f = M == -CUDART_INF_F ? 0.f : pow2(M - mn), w = ml.x == -CUDART_INF_F ? 0.f : pow2(ml.x - mn);
+        o = fmaf(o, f, w * x); L = fmaf(L, f, w * ml.y);
+        M = mn;
+    }
+    so[grp][d] = o;
+    if (d == 0) sml[grp] = make_float2(M, L);
+    __syncthreads();
+    if (grp || d >= dh) return;
+    M = -CUDART_INF_F; L = o = 0.f;
+#pragma unroll
+    for (uint32_t i = 0; i < kMergeGroups; ++i) M = fmaxf(M, sml[i].x);
+#pragma unroll
+    for (uint32_t i = 0; i < kMergeGroups; ++i) {
+        const float w = sml[i].x == -CUDART_INF_F ? 0.f : pow2(sml[i].x - M);
+        o = fmaf(w, so[i][d], o); L = fmaf(w, sml[i].y, L);
+    }
+    a.out[((size_t)(s.q0 + r / a.rep) * a.H + p.h * a.rep + r % a.rep) * dh + d] = L == 0.f ? 0.f : o / L;
+}
+
+template <typename T, int DHP, bool PAIR>
+bool go(const AttnCall& a, float* scratch, cudaStream_t st) {
+    using F = Few<T, DHP, PAIR>;
+    auto* kernel = attn_few_kernel<T, DHP, PAIR>;
+    static PerDevice<bool> ready;
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess || !ready.get(dev, [=](bool&) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)F::Smem) == cudaSuccess; }))
+        return fail("attention: shared memory attribute: %s", cudaGetErrorString(cudaGetLastError()));
+    const unsigned most = std::min(kFewCtas, (unsigned)device_sm_count() * F::PerSm);
+    const unsigned long long tiles = (unsigned long long)a.c.B * a.c.KVH * (((unsigned long long)(a.c.table ? a.c.cap : a.c.total) + kTile - 1) / kTile);
+    const unsigned grid = tiles < most ? (unsigned)std::max(tiles, 1ull) : most;
+    Part* meta = reinterpret_cast<Part*>(scratch);
+    float2* stat = reinterpret_cast<float2*>(meta + kFewCtas);
+    float* part = reinterpret_cast<float*>(stat + 2 * kFewCtas * F::Rows);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid); cfg.blockDim = dim3(32 * kWarps); cfg.dynamicSmemBytes = F::Smem; cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at; cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, kernel, a, part, stat, meta);
+    note_launch();
+    if (!check_launch("attn_few")) return false;
+    if (grid == 1) return true;
+    cfg.gridDim = dim3(grid - 1, std::min(F::Rows, a.max_q >= F::Rows ? F::Rows : a.max_q * a.rep)); cfg.blockDim = dim3(128, kMergeGroups); cfg.dynamicSmemBytes = 0;
+    cudaLaunchKernelEx(&cfg, attn_few_merge_kernel, a, (const float*)part, (const float2*)stat, (const Part*)meta, (uint32_t)F::Rows);
+    note_launch();
+    return check_launch("attn_few_merge");
+}
+
+}  // namespace
+
+size_t attn_few_scratch(uint32_t rows, uint32_t dh) {
+    const size_t slots = 2 * (size_t)kFewCtas * (rows <= 8 ? 8 : kFewRows);
+    return kFewCtas * sizeof(Part) + slots * sizeof(float2) + slots * dh * sizeof(float);
+}
+
+// a.few says how many rows a sequence has at most: up to 8 the kernel with both parts in one product
+bool launch_attn_few(const AttnCall& a, bool half, float* scratch, cudaStream_t st) {
+    const bool pair = a.few <= 8;
+    if (a.c.dh <= 64) {
+        if (half) return pair ? go<__half, 64, true>(a, scratch, st) : go<__half, 64, false>(a, scratch, st);
+        return pair ? go<float, 64, true>(a, scratch, st) : go<float, 64, false>(a, scratch, st);
+    }
+    if (half) return pair ? go<__half, 128, true>(a, scratch, st) : go<__half, 128, false>(a, scratch, st);
+    return pair ? go<float, 128, true>(a, scratch, st) : go<float, 128, false>(a, scratch, st);
+}
+
+}  // namespace tmc

@@ -1,0 +1,26 @@
+// attn_pages.h — the kernels behind tm_cuda_attn_paged_dev and tm_cuda_attn_window_dev, and which of them serves what.
+#pragma once
+
+#include "kv_pages.cuh"
+
+namespace tmc {
+
+struct AttnCall {
+    KvBatch c;
+    KvMask mask;
+    const float* q;
+    float* out;
+    uint32_t H, rep;            // query heads; of them to a K/V head
+    uint32_t max_q;             // a sequence with more new tokens is out of range
+    uint32_t few;               // rows (new tokens x rep) of a sequence up to which attn_few.cu serves it; 0: none
+    bool others;                // sequences with more rows are served by another launch of the same call
+    float scale;
+    int* status;
+};
+
+// attn_few.cu: sequences with at most 16 query rows per K/V head
+constexpr uint32_t kFewRows = 16, kFewCtas = 296;       // two CTAs on each of 148 SMs
+size_t attn_few_scratch(uint32_t rows, uint32_t dh);
+bool launch_attn_few(const AttnCall& a, bool half, float* scratch, cudaStream_t st);
+
+}  // namespace tmc
