@@ -14,7 +14,7 @@
 //   * The output is summed in fp32 registers, 16 keys at a time: a tensor core's own running sum is cut, not rounded, at every step.
 //   * A value that is masked for one row but not for another meets a weight of 0 in the product, which is NaN if the value is not
 //     finite. So a result that is not finite is computed again row by row, where masked keys are skipped.
-#include "attn_pages.h"
+#include "attn_rows.cuh"
 #include "common.cuh"
 #include "per_device.h"
 
@@ -28,11 +28,6 @@ namespace {
 
 constexpr uint32_t kWarps = 4, kTile = 64, kStep = 16;      // keys of a tile; of a warp's share of it
 
-__device__ __forceinline__ float pow2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -46,9 +41,6 @@ __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
 }
 __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
-}
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t bytes) {   // bytes 0: zeros
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
@@ -67,25 +59,17 @@ __device__ __forceinline__ void parts(float x, uint32_t& hi, uint32_t& lo) {    
 }
 
 // ---- the list of work ------------------------------------------------------------------------------------------------
-struct Unit {                       // the keys of one sequence, tile by tile: [0, a) and [b, e) in tiles that start at multiples of kTile
+struct Unit : KeyTiles<kTile> {
     KvSeq s;
-    uint32_t tiles, head_tiles, skip;        // tile t starts at key t * kTile, or (t + skip) * kTile from head_tiles on
-    uint32_t end;                   // keys from here on are behind every row's position
     bool bad;                       // its rows are NaN
 };
-__device__ __forceinline__ uint32_t tile_key(const Unit& u, uint32_t t) { return (t < u.head_tiles ? t : t + u.skip) * kTile; }
 __device__ Unit unit_of(const AttnCall& a, uint32_t b) {
     Unit u;
     u.s = kv_seq(a.c, b);
     u.bad = u.s.bad || u.s.n > a.max_q;
     const uint32_t rows = u.s.n <= a.few ? u.s.n * a.rep : a.few + 1;       // no overflow
     if (u.s.n == 0 || (rows > a.few && a.others)) { u.tiles = 0; return u; }
-    const KvSpan sp = kv_span(a.mask, u.s.first, (int)u.s.len - 1);
-    u.end = u.bad ? 0u : sp.e;
-    const uint32_t e = (u.end + kTile - 1) / kTile, lo = sp.b / kTile;
-    u.head_tiles = (sp.a + kTile - 1) / kTile;
-    u.skip = lo > u.head_tiles ? lo - u.head_tiles : 0u;
-    u.tiles = max(1u, e - min(e, u.skip));
+    u.set(kv_span(a.mask, u.s.first, (int)u.s.len - 1), u.bad);
     return u;
 }
 
@@ -99,45 +83,6 @@ template <typename T, int DHP, bool PAIR> struct Few {
     static constexpr uint32_t Smem = Ring + Merge;
     static constexpr uint32_t PerSm = Smem <= 114688 ? 2 : 1;
 };
-
-// The rows of a unit over tiles [t0, t1) once more, key by key: to part and stat, or, where the unit is all there, to out.
-template <typename T>
-__device__ __noinline__ void rows_again(const AttnCall& a, const Unit& u, uint32_t b, uint32_t h, uint32_t t0, uint32_t t1, float* part, float2* stat) {
-    const uint32_t lane = threadIdx.x & 31u, dh = a.c.dh;
-    const T* kb = (const T*)a.c.k + (size_t)h * a.c.page * dh;
-    const T* vb = (const T*)a.c.v + (size_t)h * a.c.page * dh;
-    for (uint32_t r = threadIdx.x >> 5; r < u.s.n * a.rep; r += kWarps) {
-        const int p = u.s.first + (int)(r / a.rep);
-        const size_t row = ((size_t)(u.s.q0 + r / a.rep) * a.H + h * a.rep + r % a.rep) * dh;
-        float qr[4], acc[4] = {}, m = -CUDART_INF_F, l = 0.f;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) qr[k] = lane + 32u * k < dh ? a.q[row + lane + 32u * k] * (a.scale * kLog2e) : 0.f;
-        for (uint32_t t = t0; t < t1; ++t) {
-            const uint32_t j0 = tile_key(u, t);
-            for (uint32_t j = j0; j < min(j0 + kTile, u.end); ++j) {
-                size_t at;
-                if (!kv_sees(a.mask, p, (int)j) || !kv_row(a.c, b, j, &at)) continue;
-                float x = 0.f;
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (lane + 32u * k < dh) x = fmaf(qr[k], (float)kb[at + lane + 32u * k], x);
-#pragma unroll
-                for (int s = 16; s; s >>= 1) x += __shfl_xor_sync(0xffffffffu, x, s);
-                const float mn = fmaxf(m, x), corr = m == -CUDART_INF_F ? 0.f : exp2f(m - mn), w = x == -CUDART_INF_F ? 0.f : exp2f(x - mn + kUp);
-                l = fmaf(l, corr, w);
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (lane + 32u * k < dh) acc[k] = fmaf(acc[k], corr, w * (float)vb[at + lane + 32u * k]);
-                m = mn;
-            }
-        }
-        float* to = stat ? part + (size_t)r * dh : a.out + row;
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (lane + 32u * k < dh) to[lane + 32u * k] = stat ? acc[k] : l == 0.f ? 0.f : acc[k] / l;
-        if (stat && lane == 0) stat[r] = make_float2(m, l);
-    }
-}
 
 template <typename T, int DHP, bool PAIR>
 __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_few_kernel(const __grid_constant__ AttnCall a, float* part, float2* stat, Part* meta) {
@@ -219,7 +164,7 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
     Unit lu = unit_of(a, lb);
     auto request = [&]() {
         if (left) {
-            const uint32_t j = tile_key(lu, lt) + warp * kStep + (lane & 15u);
+            const uint32_t j = lu.key(lt) + warp * kStep + (lane & 15u);
             size_t at = 0;
             const bool in = j < lu.end;
             bool ok = true;
@@ -314,7 +259,7 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
             request();
             asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
             __syncwarp();
-            const uint32_t kat = ring + use * SB, vat = kat + kStep * RB, j0 = tile_key(u, t) + warp * kStep;
+            const uint32_t kat = ring + use * SB, vat = kat + kStep * RB, j0 = u.key(t) + warp * kStep;
             if (no_page >> use & 1u) lost_page = true;
             if (j0 < u.end) {
                 float s[2][4] = {};
@@ -490,7 +435,12 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
         }
         if (bad && tid == 0) note_bad_batch(a.status);
         if (tid == 0) sm_bad[turn ^ 1u] = 0;
-        if (__syncthreads_or(again && !bad)) rows_again<T>(a, u, b, h, t0, t1, po, all ? nullptr : ps);
+        if (__syncthreads_or(again && !bad)) {
+            for (uint32_t r = warp; r < rows; r += kWarps) {
+                const size_t row = (size_t)(u.s.q0 + r / a.rep) * a.H + h * a.rep + r % a.rep;
+                row_again<T>(a, b, h, u.s.first + (int)(r / a.rep), u, t0, t1, a.q + row * dh, all ? a.out + row * dh : po + (size_t)r * dh, all ? nullptr : ps + r);
+            }
+        }
         turn ^= 1u;
         todo -= t1 - t0;
         if (!todo) return;

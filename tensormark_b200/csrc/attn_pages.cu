@@ -5,6 +5,7 @@
 #include "common.cuh"
 #include "state.h"
 
+#include <algorithm>
 #include <cmath>
 #include <cuda_fp16.h>
 #include <math_constants.h>
@@ -26,7 +27,7 @@ bool kv_batch_from(KvBatch* c, const tm_cuda_kv_pages* kv, unsigned T, unsigned 
     if (!H || H % kv->KVH || H / kv->KVH > 128) return fail("%s: %u query heads for %u K/V heads (a multiple, at most 128 each)", who, H, kv->KVH);
     if (!kv->dh || kv->dh % 8 || kv->dh > 128) return fail("%s: head dimension %u (multiples of 8 up to 128)", who, kv->dh);
     if ((uintptr_t)kv->k % 16 || (uintptr_t)kv->v % 16) return fail("%s: the pages lie on 16-byte boundaries", who);
-    if ((unsigned long long)kv->table_ld * kv->page > 0x7fffffffull || (unsigned long long)T * H > 0x7fffffffull || kv->B > 0x7ffffffu) return fail("%s: more than 2^31 - 1 positions or query rows", who);
+    if ((unsigned long long)kv->table_ld * kv->page > 0x7fffff00ull || (unsigned long long)T * H > 0x7fffffffull || kv->B > 0x7ffffffu) return fail("%s: 2^31 positions or query rows", who);
     *c = KvBatch{kv->k, kv->v, kv->table, kv->q_begin, kv->kv_len, kv->B, kv->KVH, kv->dh, kv->page, kv->npages, kv->table_ld, T, kv->table_ld * kv->page, 0u, -1};
     if ((kv->page & (kv->page - 1u)) == 0)
         for (c->page_shift = 0; 1u << c->page_shift < kv->page;) ++c->page_shift;
@@ -83,14 +84,16 @@ Split split(unsigned B, unsigned long long rows, unsigned rep) {
     return Split{B == 1 || rep > kFewRows ? 0u : rep <= 8 ? 8u : kFewRows, true};
 }
 
+size_t few_bytes(Split sp, unsigned dh) { return sp.few ? attn_few_scratch(sp.few, dh) : 0; }
+
 bool launch(AttnCall a, bool half, float* scratch, cudaStream_t st) {
     const Split sp = split(a.c.B, (unsigned long long)a.max_q * a.rep, a.rep);
     a.few = sp.few; a.others = sp.others; a.status = device_status_word();
     if (sp.few && !launch_attn_few(a, half, scratch, st)) return false;
     if (!sp.others) return true;
+    if (half) return launch_attn_chunk(a, plan_attn_chunk(a.c.T, a.c.B, a.c.KVH, a.rep, a.few), scratch + few_bytes(sp, a.c.dh) / sizeof(float), st);
     const unsigned grid = (unsigned)(((size_t)a.c.T * a.H + 3) / 4);
-    if (half) attn_rows_kernel<__half><<<grid, 128, 0, st>>>(a);
-    else attn_rows_kernel<float><<<grid, 128, 0, st>>>(a);
+    attn_rows_kernel<float><<<grid, 128, 0, st>>>(a);
     note_launch();
     return check_launch("attention");
 }
@@ -103,10 +106,11 @@ using namespace tmc;
 extern "C" {
 
 size_t tm_cuda_attn_paged_scratch(unsigned T, unsigned B, unsigned max_q, unsigned H, unsigned KVH, unsigned dh) {
-    if (!KVH || !H || H % KVH || !dh) return 0;
+    if (!KVH || !H || H % KVH || !dh || !T) return 16;
     const unsigned rep = H / KVH;
     const Split sp = split(B, (unsigned long long)(max_q && max_q < T ? max_q : T) * rep, rep);
-    return sp.few ? attn_few_scratch(sp.few, dh) : 16;
+    const size_t chunk = sp.others ? attn_chunk_scratch(plan_attn_chunk(T, B, KVH, rep, sp.few), T, H, dh) : 0;
+    return std::max<size_t>(16, few_bytes(sp, dh) + chunk);
 }
 size_t tm_cuda_attn_window_scratch(unsigned T, unsigned H, unsigned KVH, unsigned dh) { return tm_cuda_attn_paged_scratch(T, 1, T, H, KVH, dh); }
 
@@ -130,8 +134,8 @@ bool tm_cuda_attn_window_dev(const float* q, const void* kc, const void* vc, flo
     if (!q || !kc || !vc || !scratch || !out) return fail("attn_window: null pointer");
     if (!KVH || !H || H % KVH || H / KVH > 128) return fail("attn_window: %u query heads for %u K/V heads (a multiple, at most 128 each)", H, KVH);
     if (!dh || dh % 8 || dh > 128) return fail("attn_window: head dimension %u (multiples of 8 up to 128)", dh);
-    if (!ctx || ctx > 0x7fffffffu || pos0 > ctx || T > ctx - pos0) return fail("attn_window: positions %u to %llu of a cache of %u rows", pos0, (unsigned long long)pos0 + T, ctx);
-    if ((unsigned long long)T * H > 0x7fffffffull) return fail("attn_window: more than 2^31 - 1 query rows");
+    if (!ctx || ctx > 0x7fffff00u || pos0 > ctx || T > ctx - pos0) return fail("attn_window: positions %u to %llu of a cache of %u rows", pos0, (unsigned long long)pos0 + T, ctx);
+    if ((unsigned long long)T * H > 0x7fffffffull) return fail("attn_window: 2^31 query rows");
     if (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc | (uintptr_t)scratch | (uintptr_t)out) % 16) return fail("attn_window: q, the caches, scratch and out lie on 16-byte boundaries");
     if (!(scale > 0.f) || !std::isfinite(scale)) return fail("attn_window: the scale is not a positive number");
     const size_t need = tm_cuda_attn_window_scratch(T, H, KVH, dh);

@@ -23,4 +23,10 @@ constexpr uint32_t kFewRows = 16, kFewCtas = 296;       // two CTAs on each of 1
 size_t attn_few_scratch(uint32_t rows, uint32_t dh);
 bool launch_attn_few(const AttnCall& a, bool half, float* scratch, cudaStream_t st);
 
+// attn_chunk.cu: sequences with more rows, over fp16 caches
+struct ChunkPlan { uint32_t slots, splits; };           // (sequence, 256 rows) at most; parts that the keys of one are split into
+ChunkPlan plan_attn_chunk(uint32_t T, uint32_t B, uint32_t KVH, uint32_t rep, uint32_t few);
+size_t attn_chunk_scratch(const ChunkPlan& pl, uint32_t T, uint32_t H, uint32_t dh);
+bool launch_attn_chunk(const AttnCall& a, const ChunkPlan& pl, float* scratch, cudaStream_t st);
+
 }  // namespace tmc

@@ -1,0 +1,69 @@
+// attn_rows.cuh — what the two kernels behind the attention over pages share: the tiles of keys that a set of rows sees, and a row
+// computed key by key.
+#pragma once
+
+#include "attn_pages.h"
+
+#include <math_constants.h>
+
+namespace tmc {
+
+__device__ __forceinline__ float pow2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t bytes) {   // bytes 0: zeros
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+// The keys [0, a) and [b, end) in tiles of N that start at multiples of N: tile t at key t * N, from `head` on at (t + skip) * N.
+// At least one, so that rows that see nothing are visited.
+template <uint32_t N> struct KeyTiles {
+    uint32_t tiles, head, skip, end;
+    __device__ __forceinline__ void set(const KvSpan& sp, bool none) {
+        end = none ? 0u : sp.e;
+        const uint32_t e = (end + N - 1) / N, lo = sp.b / N;
+        head = (sp.a + N - 1) / N;
+        skip = lo > head ? lo - head : 0u;
+        tiles = max(1u, e - min(e, skip));
+    }
+    __device__ __forceinline__ uint32_t key(uint32_t t) const { return (t < head ? t : t + skip) * N; }
+};
+
+// One row over tiles [t0, t1) by one warp, key by key in fp32: what a kernel whose products take masked values along computes again
+// where a value was not finite. stat: the row stays unnormalised, with its maximum and sum there.
+template <typename T, uint32_t N>
+__device__ __noinline__ void row_again(const AttnCall& a, uint32_t b, uint32_t h, int p, const KeyTiles<N>& tiles, uint32_t t0, uint32_t t1, const float* q, float* to, float2* stat) {
+    const uint32_t lane = threadIdx.x & 31u, dh = a.c.dh;
+    const T* kb = (const T*)a.c.k + (size_t)h * a.c.page * dh;
+    const T* vb = (const T*)a.c.v + (size_t)h * a.c.page * dh;
+    float qr[4], acc[4] = {}, m = -CUDART_INF_F, l = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) qr[k] = lane + 32u * k < dh ? q[lane + 32u * k] * (a.scale * kLog2e) : 0.f;
+    for (uint32_t t = t0; t < t1; ++t) {
+        const uint32_t j0 = tiles.key(t);
+        for (uint32_t j = j0; j < min(j0 + N, tiles.end); ++j) {
+            size_t at;
+            if (!kv_sees(a.mask, p, (int)j) || !kv_row(a.c, b, j, &at)) continue;
+            float x = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (lane + 32u * k < dh) x = fmaf(qr[k], (float)kb[at + lane + 32u * k], x);
+#pragma unroll
+            for (int s = 16; s; s >>= 1) x += __shfl_xor_sync(0xffffffffu, x, s);
+            const float mn = fmaxf(m, x), corr = m == -CUDART_INF_F ? 0.f : exp2f(m - mn), w = x == -CUDART_INF_F ? 0.f : exp2f(x - mn + kUp);
+            l = fmaf(l, corr, w);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (lane + 32u * k < dh) acc[k] = fmaf(acc[k], corr, w * (float)vb[at + lane + 32u * k]);
+            m = mn;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (lane + 32u * k < dh) to[lane + 32u * k] = stat ? acc[k] : l == 0.f ? 0.f : acc[k] / l;
+    if (stat && lane == 0) *stat = make_float2(m, l);
+}
+
+}  // namespace tmc
