@@ -27,7 +27,8 @@ namespace tmc {
 namespace {
 
 constexpr uint32_t kRows = 128, kKeys = 128, kThreads = 384, kCols = 512;
-constexpr uint32_t kWarpMma = 0, kWarpK = 1, kWarpV = 2;     // warps 4-7 and 8-11: the rows of the two tiles
+constexpr int kNoRow = 0x7ffffffe;
+constexpr uint32_t kWarpMma = 0;                             // warps 1-3: the copies; 4-7 and 8-11: the rows of the two tiles
 
 template <int DHP> struct Chunk {
     static constexpr uint32_t Tile = kKeys * DHP * 2;      // bytes of a tile of keys, or of one part of q; 64 dims are 128 bytes
@@ -36,23 +37,37 @@ template <int DHP> struct Chunk {
     static constexpr uint32_t Smem = 4 * Tile + Buffers * Tile + 1024;        // q: two tiles of two parts
 };
 
-// K-major rows of 128 bytes, 128-byte swizzle, 8 rows 1024 bytes apart
-__device__ __forceinline__ uint64_t desc_k(uint32_t at) {
-    constexpr uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
-    return (uint64_t)hi << 32 | (uint64_t)((at & 0x3ffffu) >> 4 | 1u << 16);
+// Operand descriptors: rows of 128 bytes, 128-byte swizzle, 8 rows 1024 bytes apart. For V the rows are the summed dimension, and the
+// next 64 columns lie `half` times 16 bytes on. The low word is the place, in units of 16 bytes.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t at, uint32_t half) { return (at & 0x3ffffu) >> 4 | half << 16; }
+// Four products, A and B a fixed step apart. Fours in a loop that is not unrolled: 32 descriptors at a time are more than the issuing
+// warp's registers hold.
+template <uint32_t A_STEP, uint32_t B_STEP>
+__device__ __forceinline__ void mma4_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc, uint32_t lead) {
+    asm volatile("{\n\t.reg .pred p, q, t;\n\t.reg .b32 x, y;\n\t.reg .b64 u, v;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+                 "mov.b64 u, {%1, %8};\n\tmov.b64 v, {%2, %8};\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], u, v, %3, p;\n\t"
+                 "add.u32 x, %1, %6;\n\tadd.u32 y, %2, %7;\n\tmov.b64 u, {x, %8};\n\tmov.b64 v, {y, %8};\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], u, v, %3, t;\n\t"
+                 "add.u32 x, x, %6;\n\tadd.u32 y, y, %7;\n\tmov.b64 u, {x, %8};\n\tmov.b64 v, {y, %8};\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], u, v, %3, t;\n\t"
+                 "add.u32 x, x, %6;\n\tadd.u32 y, y, %7;\n\tmov.b64 u, {x, %8};\n\tmov.b64 v, {y, %8};\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], u, v, %3, t;\n\t}"
+                 ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(lead), "n"(A_STEP), "n"(B_STEP), "n"(kDescHi) : "memory");
 }
-// The same bytes with the rows as the summed dimension: 8 rows 1024 bytes apart, the next 64 columns `half` bytes on
-template <uint32_t HALF> __device__ __forceinline__ uint64_t desc_mn(uint32_t at) {
-    constexpr uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
-    return (uint64_t)hi << 32 | (uint64_t)((at & 0x3ffffu) >> 4 | (HALF >> 4) << 16);
-}
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t lead) {
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead) : "memory");
-}
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t lead) {
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead) : "memory");
+template <uint32_t A_STEP, uint32_t B_STEP>
+__device__ __forceinline__ void mma4_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc, uint32_t lead) {
+    asm volatile("{\n\t.reg .pred p, q, t;\n\t.reg .b32 x, y;\n\t.reg .b64 v;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+                 "mov.b64 v, {%2, %8};\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], v, %3, p;\n\t"
+                 "add.u32 x, %1, %6;\n\tadd.u32 y, %2, %7;\n\tmov.b64 v, {y, %8};\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [x], v, %3, t;\n\t"
+                 "add.u32 x, x, %6;\n\tadd.u32 y, y, %7;\n\tmov.b64 v, {y, %8};\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [x], v, %3, t;\n\t"
+                 "add.u32 x, x, %6;\n\tadd.u32 y, y, %7;\n\tmov.b64 v, {y, %8};\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [x], v, %3, t;\n\t}"
+                 ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(lead), "n"(A_STEP), "n"(B_STEP), "n"(kDescHi) : "memory");
 }
 __device__ __forceinline__ void commit(uint32_t bar, uint32_t lead) {
     asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
@@ -65,25 +80,33 @@ __device__ __forceinline__ uint32_t elect_one() {
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// A load's registers may be used behind tmem_landed, which waits for every load before it.
 __device__ __forceinline__ void tmem_ld(uint32_t t, uint32_t (&v)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
-          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
-          "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-        : "r"(t));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+                 : "r"(t));
+}
+__device__ __forceinline__ void tmem_landed(uint32_t (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31]) :: "memory");
 }
 __device__ __forceinline__ void tmem_ld(uint32_t t, uint32_t (&v)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-        : "r"(t));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                 : "r"(t));
+}
+__device__ __forceinline__ void tmem_landed(uint32_t (&v)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]) :: "memory");
+}
+__device__ __forceinline__ void tmem_ld(uint32_t t, uint32_t (&v)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "r"(t));
+}
+__device__ __forceinline__ void tmem_landed(uint32_t (&v)[8]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]) :: "memory");
 }
 __device__ __forceinline__ void tmem_st(uint32_t t, const uint32_t (&v)[16]) {
     asm volatile(
@@ -95,10 +118,17 @@ __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-// The high part is the value cut to 11 bits, so that it converts as it is; what is left has 13 and is rounded to 11.
-__device__ __forceinline__ float high_part(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
-// Is key j = j0 + i hidden from position p? lo: where p's window begins.
-__device__ __forceinline__ bool hidden(int j, int p, int lo, int sinks) { return j > p || (j < lo && j >= sinks); }
+// x, y as fp16 pairs: the rounded values, and what the rounding left, which fma's mixed form takes from the halves as they are.
+__device__ __forceinline__ void parts(float x, float y, uint32_t& hi, uint32_t& lo) {
+    float u, v;
+    hi = half2_bits(x, y);
+    asm("{\n\t.reg .b16 l, h, m;\n\tmov.b32 {l, h}, %2;\n\tmov.b16 m, 0xBC00;\n\t"
+        "fma.rn.f32.f16 %0, l, m, %3;\n\tfma.rn.f32.f16 %1, h, m, %4;\n\t}" : "=f"(u), "=f"(v) : "r"(hi), "f"(x), "f"(y));
+    lo = half2_bits(u, v);
+}
+__device__ __forceinline__ int window_from(const KvMask& m, int p) { return m.window && p >= (int)m.window ? p - (int)m.window + 1 : 0; }
+// Is key j hidden from position p, whose window begins at lo?
+__device__ __forceinline__ bool hidden(int j, int p, int lo, int sinks) { return (j > p) | ((j < lo) & (j >= sinks)); }
 
 // mbar_wait without a call in it: a row's 128 sums are live across most of these waits, more than a call may keep in registers
 __device__ __forceinline__ bool wait_for(uint64_t& bar, uint32_t parity, volatile int* gone) {
@@ -125,6 +155,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
     __shared__ uint32_t tmem_slot, unit_b, unit_tile, sums[kThreads / 32];
     __shared__ int gone, bad_page;
     __shared__ uint32_t odd[2 * kRows / 32];                 // rows that are computed again
+    __shared__ int place[2 * kRows];                         // a row's position (kNoRow: no row), needed now and then: its thread's registers are
+                                                             // full, and local memory is slow where shared memory has taken L1's place
     const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31u, tid = threadIdx.x;
     const uint32_t dh = a.c.dh;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -174,7 +206,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
 
     const uint32_t region = (smem_u32(smem_dyn) + 1023u) & ~1023u, ring = region + 4 * C::Tile;
     if (tid == 0) {
-        for (uint32_t i = 0; i < NBUF; ++i) { mbar_init(smem_u32(&bars.full[i]), 1); mbar_init(smem_u32(&bars.empty[i]), 1); }
+        for (uint32_t i = 0; i < NBUF; ++i) { mbar_init(smem_u32(&bars.full[i]), 96); mbar_init(smem_u32(&bars.empty[i]), 1); }
         for (uint32_t i = 0; i < 2; ++i) { mbar_init(smem_u32(&bars.ready[i]), 4); mbar_init(smem_u32(&bars.done[i]), 1); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -194,24 +226,25 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
             const uint32_t lead = elect_one();
             constexpr uint32_t idesc_s = (1u << 4) | ((kKeys >> 3) << 17) | ((kRows >> 4) << 24);                    // fp16 x fp16 -> fp32
             constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(DHP >> 3) << 17) | ((kRows >> 4) << 24);      // B with its rows as the summed dimension
-            auto wait_full = [&](uint32_t i) { return wait_for(bars.full[i % NBUF], i / NBUF & 1u, &gone); };
+            auto wait_full = [&](uint32_t i) {                           // the copies' writes, then the products' reads through the other proxy
+                const bool there = wait_for(bars.full[i % NBUF], i / NBUF & 1u, &gone);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                return there;
+            };
+            // The low parts first: a sum that is still small is cut to less.
             auto scores = [&](uint32_t w, uint32_t i) {                  // S of row tile w and the K tile that is the i-th in the ring
-                const uint32_t q = region + w * 2 * C::Tile, k = ring + i % NBUF * C::Tile, d = tmem + w * kKeys;
-#pragma unroll
-                for (uint32_t p = 0; p < 2; ++p)
-#pragma unroll
-                    for (uint32_t x = 0; x < DHP / 16; ++x) {
-                        const uint32_t off = (x >> 2) * C::Half + (x & 3u) * 32u;
-                        mma_ss(d, desc_k(q + p * C::Tile + off), desc_k(k + off), idesc_s, p | x, lead);
-                    }
+                const uint32_t q = desc_lo(region + w * 2 * C::Tile, 1), k = desc_lo(ring + i % NBUF * C::Tile, 1), d = tmem + w * kKeys;
+#pragma unroll 1
+                for (uint32_t x = 0; x < 2 * (DHP / 64); ++x) {          // 64 dims of one part
+                    const uint32_t off = x % (DHP / 64) * (C::Half >> 4);
+                    mma4_ss<2, 2>(d, q + (x < DHP / 64 ? C::Tile >> 4 : 0u) + off, k + off, idesc_s, x, lead);
+                }
             };
             auto values = [&](uint32_t w, uint32_t i) {                  // P V
-                const uint32_t v = ring + i % NBUF * C::Tile, pt = tmem + w * kKeys, d = tmem + 2 * kKeys + w * kKeys;
-#pragma unroll
-                for (uint32_t x = 0; x < kKeys / 16; ++x)
-#pragma unroll
-                    for (uint32_t p = 0; p < 2; ++p)
-                        mma_ts(d, pt + x * 16u + p * 8u, desc_mn<C::Half>(v + x * 2048u), idesc_o, p | x, lead);
+                const uint32_t v = desc_lo(ring + i % NBUF * C::Tile, C::Half >> 4), pt = tmem + w * kKeys, d = tmem + 2 * kKeys + w * kKeys;
+#pragma unroll 1
+                for (uint32_t x = 0; x < 4; ++x)                         // 64 keys of one part
+                    mma4_ts<16, 128>(d, pt + (x & 1u) * 64u + (x < 2 ? 8u : 0u), v + (x & 1u) * 512u, idesc_o, x, lead);
             };
             ok = wait_full(0);
             for (uint32_t w = 0; w < tiles2 && ok; ++w) {
@@ -238,38 +271,51 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
                     commit(smem_u32(&bars.done[w]), lead);
                 }
             }
-        } else if (warp == kWarpK || warp == kWarpV) {
-            const uint32_t which = warp - kWarpK, chunks = dh / 8;
-            const uint8_t* base = (const uint8_t*)(which ? a.c.v : a.c.k);
+        } else if (warp != kWarpMma) {
+            // Three warps share every tile. Offsets of K and V rows are the same; the copies arrive on the tile's barrier as they land.
+            const uint32_t mine = warp - 1, chunks = dh / 8;
+            constexpr uint32_t CH = DHP / 8, RP = 32 / CH;               // 16-byte pieces of a row, rows of a round
+            uint32_t page[4];                                            // of rows 32 r + lane of the tile after this one
             bool missing = false;
-            for (uint32_t j = 0; j < n; ++j) {
-                const uint32_t i = 2 * j + which, buf = i % NBUF, dst = ring + buf * C::Tile, j0 = kt.key(t0 + j);
+            auto slot_of = [&](uint32_t key) { return a.c.page_shift >= 0 ? key >> a.c.page_shift : key / a.c.page; };
+            auto look_up = [&](uint32_t j) {
+#pragma unroll
+                for (uint32_t r = 0; r < 4; ++r) {
+                    const uint32_t key = kt.key(t0 + j) + 32 * r + lane;
+                    page[r] = 0;
+                    if (a.c.table && j < n && key < kt.end) page[r] = (uint32_t)a.c.table[(size_t)b * a.c.table_ld + slot_of(key)];
+                }
+            };
+            look_up(0);
+            for (uint32_t j = 0; j < n && ok; ++j) {
                 uint32_t lo[4], hi[4], there[4];
 #pragma unroll
-                for (uint32_t r = 0; r < 4; ++r) {                       // the page of row 32 r + lane
-                    const uint32_t key = j0 + 32 * r + lane;
-                    size_t at = 0;
+                for (uint32_t r = 0; r < 4; ++r) {
+                    const uint32_t key = kt.key(t0 + j) + 32 * r + lane;
                     bool have = key < kt.end;
-                    if (have && !kv_row(a.c, b, key, &at)) { have = false; missing = true; }
-                    at = (at + (size_t)h * a.c.page * dh) * 2;
+                    if (have && page[r] >= a.c.npages) { have = false; missing = true; }
+                    const uint32_t row = a.c.table ? key - slot_of(key) * a.c.page : key;
+                    const size_t at = have ? (((size_t)page[r] * a.c.KVH + h) * a.c.page + row) * dh * 2 : 0;
                     lo[r] = (uint32_t)at; hi[r] = (uint32_t)(at >> 32);
                     there[r] = __ballot_sync(0xffffffffu, have);
                 }
-                if (!wait_for(bars.empty[buf], (i / NBUF & 1u) ^ 1u, &gone)) { ok = false; break; }
-                constexpr uint32_t CH = DHP / 8, RP = 32 / CH;           // 16-byte pieces of a row, rows of a round
+                look_up(j + 1);
 #pragma unroll
-                for (uint32_t r = 0; r < 4; ++r)
-#pragma unroll 8
-                    for (uint32_t k = 0; k < 32 / RP; ++k) {
-                        const uint32_t src = k * RP + lane / CH, ch = lane % CH, row = 32 * r + src;
-                        const size_t off = (size_t)__shfl_sync(0xffffffffu, lo[r], src) | (size_t)__shfl_sync(0xffffffffu, hi[r], src) << 32;
-                        const bool have = (there[r] >> src & 1u) && ch < chunks;
-                        copy16(dst + (ch >> 3) * C::Half + row * 128u + (((ch & 7u) ^ (row & 7u)) << 4), base + (have ? off + ch * 16 : 0), have ? 16u : 0u);
-                    }
-                asm volatile("cp.async.wait_all;" ::: "memory");
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                mbar_arrive_if(smem_u32(&bars.full[buf]), lane == 0);
+                for (uint32_t which = 0; which < 2; ++which) {
+                    const uint32_t i = 2 * j + which, buf = i % NBUF, dst = ring + buf * C::Tile;
+                    const uint8_t* base = (const uint8_t*)(which ? a.c.v : a.c.k);
+                    if (!wait_for(bars.empty[buf], (i / NBUF & 1u) ^ 1u, &gone)) { ok = false; break; }
+#pragma unroll
+                    for (uint32_t r = 0; r < 4; ++r)
+#pragma unroll 4
+                        for (uint32_t k = (mine + r) % 3; k < 32 / RP; k += 3) {
+                            const uint32_t src = k * RP + lane / CH, ch = lane % CH, row = 32 * r + src;
+                            const size_t off = (size_t)__shfl_sync(0xffffffffu, lo[r], src) | (size_t)__shfl_sync(0xffffffffu, hi[r], src) << 32;
+                            const bool have = (there[r] >> src & 1u) && ch < chunks;
+                            copy16(dst + (ch >> 3) * C::Half + row * 128u + (((ch & 7u) ^ (row & 7u)) << 4), base + (have ? off + ch * 16 : 0), have ? 16u : 0u);
+                        }
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(&bars.full[buf])) : "memory");
+                }
             }
             if (missing) bad_page = 1;
         }
@@ -277,100 +323,146 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const uint32_t w = (warp - 4) >> 2, r = (warp & 3u) * 32 + lane, row = w * kRows + r;
         if (w < tiles2) {
-            const bool is = row < rows;
-            const uint32_t gi = row0 + (is ? row : 0u), tok = gi / a.rep;
-            const size_t at = ((size_t)(s.q0 + tok) * a.H + h * a.rep + gi % a.rep) * dh;
-            const int p = is ? s.first + (int)tok : 0x7ffffffe, lo = a.mask.window && p >= (int)a.mask.window ? p - (int)a.mask.window + 1 : 0, sinks = (int)a.mask.sinks;
-            // rows that are none see everything, so that they ask for no masks
-            const int p_min = __reduce_min_sync(0xffffffffu, p), lo_max = __reduce_max_sync(0xffffffffu, is ? lo : 0);
-            float back;
+            auto number_of = [&](uint32_t i) {                           // of the row in q and out
+                const uint32_t tok = (uint32_t)(place[i] - s.first);
+                return (size_t)(s.q0 + tok) * a.H + h * a.rep + (row0 + i - tok * a.rep);
+            };
+            int p_min, lo_max;                                           // the least that a row of the warp sees ahead and behind
             {
-                float top = 0.f;
-                for (uint32_t d = 0; d < dh; d += 4) {
-                    const float4 f = is ? *reinterpret_cast<const float4*>(a.q + at + d) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    top = fmaxf(fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y))), fmaxf(fabsf(f.z), fabsf(f.w)));
-                }
-                top *= a.scale * kLog2e;
-                const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 120);          // the row's largest to [2^13, 2^14)
-                const float up = __uint_as_float((uint32_t)(127 + 13 - e) << 23);
-                back = __uint_as_float((uint32_t)(127 - 13 + e) << 23);
-#pragma unroll 4
-                for (uint32_t c = 0; c < DHP / 8; ++c) {
-                    float f[8];
-#pragma unroll
-                    for (uint32_t k = 0; k < 8; k += 4) {
-                        const float4 x = is && c * 8 < dh ? *reinterpret_cast<const float4*>(a.q + at + c * 8 + k) : make_float4(0.f, 0.f, 0.f, 0.f);
-                        f[k] = x.x; f[k + 1] = x.y; f[k + 2] = x.z; f[k + 3] = x.w;
-                    }
-                    uint32_t hi[4], low[4];
-#pragma unroll
-                    for (uint32_t k = 0; k < 4; ++k) {
-                        const float x = f[2 * k] * (a.scale * kLog2e) * up, y = f[2 * k + 1] * (a.scale * kLog2e) * up, xh = high_part(x), yh = high_part(y);
-                        hi[k] = half2_bits(xh, yh); low[k] = half2_bits(x - xh, y - yh);
-                    }
-                    const uint32_t to = region + w * 2 * C::Tile + (c >> 3) * C::Half + r * 128u + (((c & 7u) ^ (r & 7u)) << 4);
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + C::Tile), "r"(low[0]), "r"(low[1]), "r"(low[2]), "r"(low[3]) : "memory");
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                mbar_arrive_if(smem_u32(&bars.ready[w]), lane == 0);
+                const bool is = row < rows;
+                const uint32_t gi = row0 + (is ? row : 0u), tok = gi / a.rep;
+                const int p = is ? s.first + (int)tok : kNoRow;          // rows that are none see everything, so that they ask for no masks
+                place[row] = p;
+                p_min = __reduce_min_sync(0xffffffffu, p);
+                lo_max = __reduce_max_sync(0xffffffffu, is ? window_from(a.mask, p) : 0);
             }
+            // q: a row per turn (two for heads of 64), four dims per lane, so that the loads are whole lines
+            constexpr uint32_t LR = DHP / 4, RT = 32 / LR;               // lanes of a row, rows of a turn
+            const uint32_t first_row = row - lane, piece = lane % LR;
+            float back = 1.f;
+            __syncwarp();
+            constexpr uint32_t AHEAD = 16;                               // turns whose loads are on their way together
+            const float by = a.scale * kLog2e;
+#pragma unroll 1
+            for (uint32_t i0 = 0; i0 < 32; i0 += AHEAD * RT) {
+                float4 ahead[AHEAD];
+#pragma unroll
+                for (uint32_t n1 = 0; n1 < AHEAD; ++n1) {
+                    const uint32_t rr = first_row + i0 + n1 * RT + lane / LR;
+                    ahead[n1] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (rr < rows && 4 * piece < dh) ahead[n1] = *reinterpret_cast<const float4*>(a.q + number_of(rr) * dh + 4 * piece);
+                }
+#pragma unroll
+                for (uint32_t n1 = 0; n1 < AHEAD; ++n1) {
+                    const uint32_t i = i0 + n1 * RT, rq = (first_row + i + lane / LR) % kRows;
+                    const float4 f = ahead[n1];
+                    float top = fmaxf(fmaxf(fabsf(f.x), fabsf(f.y)), fmaxf(fabsf(f.z), fabsf(f.w))) * by;
+#pragma unroll
+                    for (uint32_t x = LR / 2; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                    const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 120);      // the row's largest to [2^13, 2^14)
+                    const float up = __uint_as_float((uint32_t)(127 + 13 - e) << 23);
+                    uint32_t hi[2], low[2];
+                    parts(f.x * by * up, f.y * by * up, hi[0], low[0]);
+                    parts(f.z * by * up, f.w * by * up, hi[1], low[1]);
+                    const uint32_t c = piece / 2, to = region + w * 2 * C::Tile + (c >> 3) * C::Half + rq * 128u + (((c & 7u) ^ (rq & 7u)) << 4) + (piece & 1u) * 8u;
+                    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to), "r"(hi[0]), "r"(hi[1]) : "memory");
+                    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to + C::Tile), "r"(low[0]), "r"(low[1]) : "memory");
+#pragma unroll
+                    for (uint32_t k = 0; k < RT; ++k) {
+                        const int es = __shfl_sync(0xffffffffu, e, k * LR);
+                        if (lane == i + k) back = __uint_as_float((uint32_t)(127 - 13 + es) << 23);
+                    }
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            mbar_arrive_if(smem_u32(&bars.ready[w]), lane == 0);
             const uint32_t lanes = (warp & 3u) << 21, st = tmem + w * kKeys + lanes, ot = tmem + 2 * kKeys + w * kKeys + lanes;
             float o[DHP], m = -CUDART_INF_F, l = 0.f, corr = 0.f;
 #pragma unroll
             for (uint32_t d = 0; d < DHP; ++d) o[d] = 0.f;
-            auto add_values = [&]() {                                    // O = O corr + P V
+            {                                                            // what the first tile finds as the values of the one before
+                uint32_t none[16] = {};
 #pragma unroll
-                for (uint32_t c = 0; c < DHP / 32; ++c) {
-                    uint32_t v[32];
-                    tmem_ld(ot + 32 * c, v);
+                for (uint32_t d = 0; d < DHP; d += 16) tmem_st(ot + d, none);
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            }
+            // S of the tiles that not every row of the warp sees whole: what a row does not see is -infinity from here on
+            auto hide = [&](int j0) {
+                const int p = place[row], lo = window_from(a.mask, p), sinks = (int)a.mask.sinks;
+#pragma unroll 1
+                for (uint32_t c = 0; c < kKeys / 16; ++c) {
+                    const int i0 = j0 + (int)(16 * c);
+                    if (i0 + 15 <= p_min && (i0 >= lo_max || i0 + 16 <= sinks)) continue;
+                    uint32_t v[16];
+                    tmem_ld(st + 16 * c, v);
+                    tmem_landed(v);
 #pragma unroll
-                    for (uint32_t k = 0; k < 32; ++k) o[32 * c + k] = fmaf(o[32 * c + k], corr, __uint_as_float(v[k]));
+                    for (uint32_t k = 0; k < 16; ++k)
+                        v[k] = hidden(i0 + (int)k, p, lo, sinks) ? 0xff800000u : v[k];
+                    tmem_st(st + 16 * c, v);
                 }
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            };
+            auto maximum = [&]() {
+                float top[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+                uint32_t v[2][16];
+                tmem_ld(st, v[0]);
+#pragma unroll
+                for (uint32_t c = 0; c < kKeys / 16; ++c) {
+                    tmem_landed(v[c & 1]);
+                    if (c + 1 < kKeys / 16) tmem_ld(st + 16 * (c + 1), v[(c + 1) & 1]);
+#pragma unroll
+                    for (uint32_t k = 0; k < 16; ++k) top[k & 3u] = fmaxf(top[k & 3u], __uint_as_float(v[c & 1][k]));
+                }
+                return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            };
+            // S in, P out, the sum on the way; and, since the exponentials leave the other pipes idle, P V of the tile before into O. The
+            // exponentials of 8 keys are under way while the 8 before them are split and stored.
+            auto weights = [&](float base, float now) {
+                constexpr uint32_t N = kKeys / 8;
+                const float shift = kUp - base;
+                float sum[4] = {}, y[2][8];
+                uint32_t v[8], x[16], z[8];
+                tmem_ld(st, v);
+                tmem_landed(v);
+#pragma unroll
+                for (uint32_t k = 0; k < 8; ++k) y[0][k] = pow2(fmaf(__uint_as_float(v[k]), back, shift));
+                tmem_ld(st + 8, v);
+                tmem_ld(ot, z);
+#pragma unroll
+                for (uint32_t c = 0; c < N; ++c) {
+                    const uint32_t g = 4 * (c & 1u);
+                    tmem_landed(v);
+                    if (c + 1 < N) {
+#pragma unroll
+                        for (uint32_t k = 0; k < 8; ++k) y[(c + 1) & 1][k] = pow2(fmaf(__uint_as_float(v[k]), back, shift));
+                    }
+                    if (c < DHP / 8) {
+                        tmem_landed(z);
+#pragma unroll
+                        for (uint32_t k = 0; k < 8; ++k) o[8 * c + k] = fmaf(o[8 * c + k], corr, __uint_as_float(z[k]));
+                    }
+                    if (c + 2 < N) tmem_ld(st + 8 * (c + 2), v);
+                    if (c + 1 < DHP / 8) tmem_ld(ot + 8 * (c + 1), z);
+#pragma unroll
+                    for (uint32_t k = 0; k < 8; k += 2) {
+                        sum[k >> 1] += y[c & 1][k] + y[c & 1][k + 1];
+                        parts(y[c & 1][k], y[c & 1][k + 1], x[g + (k >> 1)], x[8 + g + (k >> 1)]);
+                    }
+                    if (c & 1u) tmem_st(st + 8 * (c - 1), x);
+                }
+                l = fmaf(l, now, (sum[0] + sum[1]) + (sum[2] + sum[3]));
             };
             for (uint32_t j = 0; j < n; ++j) {
                 if (!wait_for(bars.done[w], j & 1u, &gone)) { ok = false; break; }
                 fence_after();
                 const int j0 = (int)kt.key(t0 + j);
-                const bool whole = j0 + (int)kKeys - 1 <= p_min && (j0 >= lo_max || j0 + (int)kKeys <= sinks);
-                float top = -CUDART_INF_F;
-#pragma unroll
-                for (uint32_t c = 0; c < 4; ++c) {
-                    uint32_t v[32];
-                    tmem_ld(st + 32 * c, v);
-                    if (!whole) {
-#pragma unroll
-                        for (uint32_t k = 0; k < 32; ++k)
-                            if (hidden(j0 + (int)(32 * c + k), p, lo, sinks)) v[k] = 0xff800000u;
-                    }
-#pragma unroll
-                    for (uint32_t k = 0; k < 32; ++k) top = fmaxf(top, __uint_as_float(v[k]));
-                }
-                const float mn = fmaxf(m, top * back), base = mn == -CUDART_INF_F ? 0.f : mn, now = pow2(m - base);
+                const bool whole = j0 + (int)kKeys - 1 <= p_min && (j0 >= lo_max || j0 + (int)kKeys <= (int)a.mask.sinks);
+                if (!whole) hide(j0);
+                const float mn = fmaxf(m, maximum() * back), base = mn == -CUDART_INF_F ? 0.f : mn, now = pow2(m - base);
                 m = mn;
-                const float shift = kUp - base;
-                float sum[4] = {};
-#pragma unroll
-                for (uint32_t c = 0; c < kKeys / 16; ++c) {
-                    uint32_t v[16], x[16];
-                    tmem_ld(st + 16 * c, v);
-#pragma unroll
-                    for (uint32_t k = 0; k < 16; k += 2) {
-                        float y = pow2(fmaf(__uint_as_float(v[k]), back, shift)), z = pow2(fmaf(__uint_as_float(v[k + 1]), back, shift));
-                        if (!whole) {
-                            if (hidden(j0 + (int)(16 * c + k), p, lo, sinks)) y = 0.f;
-                            if (hidden(j0 + (int)(16 * c + k + 1), p, lo, sinks)) z = 0.f;
-                        }
-                        sum[k >> 1 & 3u] += y + z;
-                        const float yh = high_part(y), zh = high_part(z);
-                        x[k >> 1] = half2_bits(yh, zh);
-                        x[8 + (k >> 1)] = half2_bits(y - yh, z - zh);
-                    }
-                    tmem_st(st + 16 * c, x);
-                }
-                l = fmaf(l, now, (sum[0] + sum[1]) + (sum[2] + sum[3]));
-                if (j) add_values();
+                weights(base, now);
                 corr = now;
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 fence_before();
@@ -378,23 +470,43 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
                 mbar_arrive_if(smem_u32(&bars.ready[w]), lane == 0);
             }
             if (n && ok) {
-                if (wait_for(bars.done[w], n & 1u, &gone)) { fence_after(); add_values(); }
+                if (wait_for(bars.done[w], n & 1u, &gone)) {
+                    fence_after();
+#pragma unroll
+                    for (uint32_t c = 0; c < DHP / 32; ++c) {
+                        uint32_t v[32];
+                        tmem_ld(ot + 32 * c, v);
+                        tmem_landed(v);
+#pragma unroll
+                        for (uint32_t k = 0; k < 32; ++k) o[32 * c + k] = fmaf(o[32 * c + k], corr, __uint_as_float(v[k]));
+                    }
+                }
                 else ok = false;
             }
             bool finite = fabsf(l) < CUDART_INF_F;
 #pragma unroll
             for (uint32_t d = 0; d < DHP; ++d) finite = finite && fabsf(o[d]) < CUDART_INF_F;
             if (!ok || bad) l = CUDART_NAN_F;
+            const bool is = place[row] != kNoRow;
             const uint32_t again = __ballot_sync(0xffffffffu, is && ok && !bad && !finite);
             if (lane == 0) odd[w * 4 + (warp & 3u)] = again;
-            if (is) {
-                const size_t to = splits > 1 ? ((size_t)split * a.c.T * a.H) * dh + at : at;
-                float* out = (splits > 1 ? part : a.out) + to;
-                const float by = splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+            // out: through shared memory (q's, which no product reads any more), so that the stores are whole lines
+            const float inv = splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+            const uint32_t stage = region + w * 2 * C::Tile;
 #pragma unroll
-                for (uint32_t d = 0; d < DHP; d += 4)
-                    if (d < dh) *reinterpret_cast<float4*>(out + d) = make_float4(o[d] * by, o[d + 1] * by, o[d + 2] * by, o[d + 3] * by);
-                if (splits > 1) stat[to / dh] = make_float2(m, l);
+            for (uint32_t c = 0; c < LR; ++c)
+                asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(stage + r * (DHP * 4) + ((c ^ (r % LR)) << 4)),
+                             "f"(o[4 * c] * inv), "f"(o[4 * c + 1] * inv), "f"(o[4 * c + 2] * inv), "f"(o[4 * c + 3] * inv) : "memory");
+            __syncwarp();
+            const size_t shift = splits > 1 ? (size_t)split * a.c.T * a.H : 0;
+            float* const out = splits > 1 ? part : a.out;
+            if (is && splits > 1) stat[shift + number_of(row)] = make_float2(m, l);
+#pragma unroll 8
+            for (uint32_t i = 0; i < 32; i += RT) {
+                const uint32_t rr = first_row + i + lane / LR, rq = rr % kRows;
+                float4 f;
+                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(stage + rq * (DHP * 4) + ((piece ^ (rq % LR)) << 4)) : "memory");
+                if (rr < rows && 4 * piece < dh) *reinterpret_cast<float4*>(out + (shift + number_of(rr)) * dh + 4 * piece) = f;
             }
         }
     }

@@ -34,7 +34,7 @@ template <uint32_t N> struct KeyTiles {
 // One row over tiles [t0, t1) by one warp, key by key in fp32: what a kernel whose products take masked values along computes again
 // where a value was not finite. stat: the row stays unnormalised, with its maximum and sum there.
 template <typename T, uint32_t N>
-__device__ __noinline__ void row_again(const AttnCall& a, uint32_t b, uint32_t h, int p, const KeyTiles<N>& tiles, uint32_t t0, uint32_t t1, const float* q, float* to, float2* stat) {
+__device__ __noinline__ void row_again(const AttnCall& a, uint32_t b, uint32_t h, int p, KeyTiles<N> tiles, uint32_t t0, uint32_t t1, const float* q, float* to, float2* stat) {
     const uint32_t lane = threadIdx.x & 31u, dh = a.c.dh;
     const T* kb = (const T*)a.c.k + (size_t)h * a.c.page * dh;
     const T* vb = (const T*)a.c.v + (size_t)h * a.c.page * dh;
