@@ -18,6 +18,7 @@
 #include "attn_rows.cuh"
 #include "bulk.cuh"
 #include "common.cuh"
+#include "pdl.cuh"
 #include "per_device.h"
 
 #include <algorithm>
@@ -26,7 +27,7 @@
 namespace tmc {
 namespace {
 
-constexpr uint32_t kRows = 128, kKeys = 128, kThreads = 384, kCols = 512;
+constexpr uint32_t kRows = kChunkRows / 2, kKeys = 128, kThreads = 384, kCols = 512;
 constexpr int kNoRow = 0x7ffffffe;
 constexpr uint32_t kWarpMma = 0;                             // warps 1-3: the copies; 4-7 and 8-11: the rows of the two tiles
 
@@ -159,8 +160,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
                                                              // full, and local memory is slow where shared memory has taken L1's place
     const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31u, tid = threadIdx.x;
     const uint32_t dh = a.c.dh;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    pdl_enter();
 
     // ---- which sequence, and which of its row tiles: counted from the last one (the longest of a prompt) ----
     const uint32_t at_once = a.c.KVH * splits, slot = (gridDim.x - 1 - blockIdx.x) / at_once, h = blockIdx.x % at_once % a.c.KVH, split = blockIdx.x % at_once / a.c.KVH;
@@ -540,15 +540,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
 
 // A warp per row: its parts, weighted by their maxima.
 __global__ void __launch_bounds__(256) attn_chunk_merge_kernel(const __grid_constant__ AttnCall a, uint32_t splits, const float* part, const float2* stat) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    pdl_enter();
     const uint32_t lane = threadIdx.x & 31u, dh = a.c.dh;
     const size_t rows = (size_t)a.c.T * a.H, row = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (row >= rows) return;
-    const uint32_t t = (uint32_t)(row / a.H), b = kv_find_seq(a.c, t);
-    if (b >= a.c.B) return;
-    const KvSeq s = kv_seq(a.c, b);
-    if (s.lost || t < s.q0 || t - s.q0 >= s.n || (unsigned long long)s.n * a.rep <= a.few) return;
+    uint32_t b;
+    KvSeq s;
+    if (!kv_find_seq(a.c, (uint32_t)(row / a.H), &b, &s) || s.n * a.rep <= a.few) return;
     float M = -CUDART_INF_F, L = 0.f;
     for (uint32_t i = 0; i < splits; ++i) M = fmaxf(M, stat[i * rows + row].x);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -577,28 +575,24 @@ bool go(const AttnCall& a, const ChunkPlan& pl, float* scratch, cudaStream_t st)
     const size_t rows = (size_t)a.c.T * a.H;
     float* part = scratch;
     float2* stat = reinterpret_cast<float2*>(part + pl.splits * rows * a.c.dh);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)ctas); cfg.blockDim = dim3(kThreads); cfg.dynamicSmemBytes = Chunk<DHP>::Smem; cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at; cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, kernel, a, pl.splits, part, stat);
+    launch_overlapped(kernel, dim3((unsigned)ctas), dim3(kThreads), Chunk<DHP>::Smem, st, a, pl.splits, part, stat);
     note_launch();
     if (!check_launch("attn_chunk")) return false;
-    if (pl.splits == 1) return true;
-    cfg.gridDim = dim3((unsigned)((rows + 7) / 8)); cfg.blockDim = dim3(256); cfg.dynamicSmemBytes = 0;
-    cudaLaunchKernelEx(&cfg, attn_chunk_merge_kernel, a, pl.splits, (const float*)part, (const float2*)stat);
-    note_launch();
-    return check_launch("attn_chunk_merge");
+    return pl.splits == 1 || launch_attn_merge(a, pl.splits, part, stat, st);
 }
 
 }  // namespace
 
-ChunkPlan plan_attn_chunk(uint32_t T, uint32_t B, uint32_t KVH, uint32_t rep, uint32_t few) {
-    const unsigned long long rows = (unsigned long long)T * rep, least = (rows + 2 * kRows - 1) / (2 * kRows);
+bool launch_attn_merge(const AttnCall& a, uint32_t splits, const float* part, const float2* stat, cudaStream_t st) {
+    launch_overlapped(attn_chunk_merge_kernel, dim3((unsigned)(((size_t)a.c.T * a.H + 7) / 8)), dim3(256), 0, st, a, splits, part, stat);
+    note_launch();
+    return check_launch("attn_chunk_merge");
+}
+
+ChunkPlan plan_attn_chunk(uint32_t T, uint32_t B, uint32_t KVH, uint32_t rep, uint32_t few, uint32_t row_tile) {
+    const unsigned long long rows = (unsigned long long)T * rep, least = (rows + row_tile - 1) / row_tile;
     ChunkPlan pl;
-    pl.slots = (uint32_t)(rows / (2 * kRows) + std::min<unsigned long long>(B, rows / (few + 1ull)));
+    pl.slots = (uint32_t)(rows / row_tile + std::min<unsigned long long>(B, rows / (few + 1ull)));
     pl.splits = (uint32_t)std::max<unsigned long long>(1, std::min<unsigned long long>(148 / (least * KVH), 16));
     return pl;
 }

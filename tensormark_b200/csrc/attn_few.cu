@@ -16,6 +16,7 @@
 //     finite. So a result that is not finite is computed again row by row, where masked keys are skipped.
 #include "attn_rows.cuh"
 #include "common.cuh"
+#include "pdl.cuh"
 #include "per_device.h"
 
 #include <algorithm>
@@ -63,10 +64,20 @@ struct Unit : KeyTiles<kTile> {
     KvSeq s;
     bool bad;                       // its rows are NaN
 };
-__device__ Unit unit_of(const AttnCall& a, uint32_t b) {
+__device__ __forceinline__ uint32_t row_tiles(const AttnCall& a, uint32_t b, bool note) {        // 16 rows each, of a sequence with more than `few`
+    const KvSeq s = kv_seq(a.c, b);
+    if (s.lost && note) note_bad_batch(a.status);
+    return s.n * a.rep <= a.few ? 0u : (s.n * a.rep + kFewRows - 1) / kFewRows;
+}
+// The rows of sequence b together (r0 = 0 and not more than `few`), or 16 of them from r0 on
+__device__ Unit unit_of(const AttnCall& a, uint32_t b, uint32_t r0) {
     Unit u;
     u.s = kv_seq(a.c, b);
     u.bad = u.s.bad || u.s.n > a.max_q;
+    if (a.tiled) {
+        u.set(kv_span(a.mask, u.s.first + (int)(r0 / a.rep), u.s.first + (int)((min(r0 + kFewRows, u.s.n * a.rep) - 1) / a.rep)), u.bad);
+        return u;
+    }
     const uint32_t rows = u.s.n <= a.few ? u.s.n * a.rep : a.few + 1;       // no overflow
     if (u.s.n == 0 || (rows > a.few && a.others)) { u.tiles = 0; return u; }
     u.set(kv_span(a.mask, u.s.first, (int)u.s.len - 1), u.bad);
@@ -84,8 +95,10 @@ template <typename T, int DHP, bool PAIR> struct Few {
     static constexpr uint32_t PerSm = Smem <= 114688 ? 2 : 1;
 };
 
-template <typename T, int DHP, bool PAIR>
-__global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_few_kernel(const __grid_constant__ AttnCall a, float* part, float2* stat, Part* meta) {
+// TILED: sequences with more rows than `few`, 16 rows of one per CTA and a share of its keys, `splits` shares; the parts go to part and
+// stat by the number of the row. Else the stretches of the list.
+template <typename T, int DHP, bool PAIR, bool TILED>
+__global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_few_kernel(const __grid_constant__ AttnCall a, float* part, float2* stat, Part* meta, uint32_t splits) {
     using F = Few<T, DHP, PAIR>;
     constexpr bool kHalf = sizeof(T) == 2;
     constexpr uint32_t RB = F::RowBytes, SB = F::StageBytes, S = F::Stages, ROWS = F::Rows, NB = DHP / 8, NR = PAIR ? 1 : 2;
@@ -96,17 +109,46 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
     __shared__ float sm_m[kWarps][ROWS], sm_l[kWarps][ROWS];
     __shared__ int sm_bad[2];
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g = lane >> 2, t4 = lane & 3u;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    pdl_enter();
     const uint32_t dh = a.c.dh, KVH = a.c.KVH;
 
     // ---- this CTA's stretch of the list ----
     unsigned long long x0, x1, total;
-    {
+    uint32_t r0 = 0;                                        // TILED: its first row
+    Unit u0;
+    if constexpr (TILED) {
+        const uint32_t at_once = KVH * splits, slot = (gridDim.x - 1 - blockIdx.x) / at_once, split = blockIdx.x % at_once / KVH;
+        if (tid == 0) { at_b = a.c.B; at_h = blockIdx.x % at_once % KVH; sm_bad[0] = sm_bad[1] = 0; }
+        const uint32_t per = (a.c.B + blockDim.x - 1) / blockDim.x, b0 = min(a.c.B, tid * per), b1 = min(a.c.B, b0 + per);
+        uint32_t mine = 0;
+        for (uint32_t b = b0; b < b1; ++b) mine += row_tiles(a, b, blockIdx.x == 0);
+        uint32_t incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= (uint32_t)o) incl += y; }
+        if (lane == 31) sums[warp] = incl;
+        __syncthreads();
+        uint32_t before = incl - mine;
+        for (uint32_t w = 0; w < warp; ++w) before += (uint32_t)sums[w];
+        if (slot >= before && slot < before + mine)
+            for (uint32_t b = b0; b < b1; ++b) {
+                const uint32_t n = row_tiles(a, b, false);
+                if (slot < before + n) { at_b = b; at_t = slot - before; break; }
+                before += n;
+            }
+        __syncthreads();
+        if (at_b == a.c.B) return;
+        r0 = at_t * kFewRows;
+        u0 = unit_of(a, at_b, r0);
+        x0 = (unsigned long long)u0.tiles * split / splits; x1 = (unsigned long long)u0.tiles * (split + 1) / splits;
+        part += (size_t)split * a.c.T * a.H * dh; stat += (size_t)split * a.c.T * a.H;
+        __syncthreads();
+        if (tid == 0) at_t = (uint32_t)x0;
+        __syncthreads();
+    } else {
         const uint32_t per = (a.c.B + blockDim.x - 1) / blockDim.x, b0 = min(a.c.B, tid * per), b1 = min(a.c.B, b0 + per);
         unsigned long long mine = 0;
         for (uint32_t b = b0; b < b1; ++b) {
-            const Unit u = unit_of(a, b);
+            const Unit u = unit_of(a, b, 0);
             if (u.s.lost && blockIdx.x == 0) note_bad_batch(a.status);
             mine += (unsigned long long)u.tiles * KVH;
         }
@@ -125,7 +167,7 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
         unsigned long long x = before + incl - mine;
         if (x0 >= x && x0 < x + mine) {                     // the stretch begins in one of this thread's sequences
             for (uint32_t b = b0; b < b1; ++b) {
-                const Unit u = unit_of(a, b);
+                const Unit u = unit_of(a, b, 0);
                 const unsigned long long n = (unsigned long long)u.tiles * KVH;
                 if (x0 < x + n) {
                     const uint32_t h = (uint32_t)((x0 - x) / u.tiles), t = (uint32_t)((x0 - x) % u.tiles);
@@ -161,7 +203,7 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
     // ---- the copies: a cursor of their own, Stages - 1 tiles ahead ----
     uint32_t lb = at_b, lh = at_h, lt = at_t, left = (uint32_t)(x1 - x0), slot = 0;
     uint32_t no_page = 0;                                   // bit of a stage: a page was not there
-    Unit lu = unit_of(a, lb);
+    Unit lu = TILED ? u0 : unit_of(a, lb, 0);
     auto request = [&]() {
         if (left) {
             const uint32_t j = lu.key(lt) + warp * kStep + (lane & 15u);
@@ -191,7 +233,7 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
                 if (++lh == KVH) {
                     lh = 0;
                     lu.tiles = 0;
-                    while (lu.tiles == 0 && ++lb < a.c.B) lu = unit_of(a, lb);
+                    while (lu.tiles == 0 && ++lb < a.c.B) lu = unit_of(a, lb, 0);
                     if (lb >= a.c.B) left = 0;              // the arrays are not what they were: nothing behind them is read
                 }
             }
@@ -202,11 +244,15 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
 #pragma unroll
     for (uint32_t i = 0; i + 1 < S; ++i) request();
 
+    auto number_of = [&](const Unit& u, uint32_t h, uint32_t r) {        // of a row of a unit in q and out
+        const uint32_t i = r / a.rep;
+        return (size_t)(u.s.q0 + i) * a.H + h * a.rep + (r - i * a.rep);
+    };
     // ---- the units of the stretch ----
     uint32_t b = at_b, h = at_h, t = at_t, todo = (uint32_t)(x1 - x0), use = 0, turn = 0;
-    Unit u = unit_of(a, b);
+    Unit u = TILED ? u0 : unit_of(a, b, 0);
     for (;;) {
-        const uint32_t t0 = t, t1 = min(u.tiles, t + todo), rows = min(u.s.n * a.rep, ROWS);
+        const uint32_t t0 = t, t1 = min(u.tiles, t + todo), rows = min(u.s.n * a.rep - r0, ROWS);
         int pos[NR];
         float back[NR], m[NR], l[NR], o[NB][2 * NR];        // back: what undoes q's power of two
         uint32_t qf[NR][KS][4];                             // fp16: the fragments, both parts; fp32: the values of a row
@@ -214,10 +260,10 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
             const float* qp[NR];
 #pragma unroll
             for (uint32_t n = 0; n < NR; ++n) {
-                const uint32_t r = g + 8 * n, i = r / a.rep;
-                const bool is = r < rows;
+                const uint32_t r = r0 + g + 8 * n, i = r / a.rep;
+                const bool is = g + 8 * n < rows;
                 pos[n] = is ? u.s.first + (int)i : -1;
-                qp[n] = is ? a.q + ((size_t)(u.s.q0 + i) * a.H + h * a.rep + r % a.rep) * dh : nullptr;
+                qp[n] = is ? a.q + number_of(u, h, r) * dh : nullptr;
                 m[n] = -CUDART_INF_F; l[n] = 0.f; back[n] = 1.f;
                 float2 raw[2 * KS];
 #pragma unroll
@@ -254,6 +300,7 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
 #pragma unroll
             for (uint32_t k = 0; k < 2 * NR; ++k) o[i][k] = 0.f;
         bool lost_page = false;
+        const int p_least = u.s.first + (int)(r0 / a.rep);
 
         for (; t < t1; ++t) {
             request();
@@ -297,8 +344,8 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
                         }
                     }
                 }
-                const bool whole = (int)j0 + (int)kStep - 1 <= u.s.first &&
-                                   (!a.mask.window || j0 + a.mask.window >= u.s.len || j0 + kStep <= a.mask.sinks);
+                const bool whole = (int)j0 + (int)kStep - 1 <= p_least &&
+                                   (!a.mask.window || j0 + a.mask.window >= u.end || j0 + kStep <= a.mask.sinks);
                 float corr[NR];
                 uint32_t ph[NR][4];                         // the weights as the second product's rows: PAIR: [0] both parts; else high, low
 #pragma unroll
@@ -405,7 +452,7 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
         }
         if ((lost_page || u.bad) && lane == 0) sm_bad[turn] = 1;
         __syncthreads();
-        const bool bad = sm_bad[turn], all = t0 == 0 && t1 == u.tiles;
+        const bool bad = sm_bad[turn], all = TILED ? splits == 1 : t0 == 0 && t1 == u.tiles;
         const size_t slot = 2 * (size_t)blockIdx.x + (t0 == 0);            // of a unit that began before: 0; that goes on behind: 1
         float* const po = part + slot * ROWS * dh;
         float2* const ps = stat + slot * ROWS;
@@ -424,21 +471,25 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
                 again = again || !(fabsf(x) < CUDART_INF_F) || !(fabsf(L) < CUDART_INF_F);
                 if (bad) L = CUDART_NAN_F;
                 if (all) {
-                    a.out[((size_t)(u.s.q0 + r / a.rep) * a.H + h * a.rep + r % a.rep) * dh + tid] = L == 0.f ? 0.f : x / L;
+                    a.out[number_of(u, h, r0 + r) * dh + tid] = L == 0.f ? 0.f : x / L;
+                } else if (TILED) {
+                    part[number_of(u, h, r0 + r) * dh + tid] = x;
+                    if (tid == 0) stat[number_of(u, h, r0 + r)] = make_float2(M, L);
                 } else {
                     po[(size_t)r * dh + tid] = x;
                     if (tid == 0) ps[r] = make_float2(M, L);
                 }
             }
-            if (bad)                                        // more rows than were promised
-                for (uint32_t r = rows; r < u.s.n * a.rep; ++r) a.out[((size_t)(u.s.q0 + r / a.rep) * a.H + h * a.rep + r % a.rep) * dh + tid] = CUDART_NAN_F;
+            if (!TILED && bad)                              // more rows than were promised
+                for (uint32_t r = rows; r < u.s.n * a.rep; ++r) a.out[number_of(u, h, r) * dh + tid] = CUDART_NAN_F;
         }
         if (bad && tid == 0) note_bad_batch(a.status);
         if (tid == 0) sm_bad[turn ^ 1u] = 0;
         if (__syncthreads_or(again && !bad)) {
             for (uint32_t r = warp; r < rows; r += kWarps) {
-                const size_t row = (size_t)(u.s.q0 + r / a.rep) * a.H + h * a.rep + r % a.rep;
-                row_again<T>(a, b, h, u.s.first + (int)(r / a.rep), u, t0, t1, a.q + row * dh, all ? a.out + row * dh : po + (size_t)r * dh, all ? nullptr : ps + r);
+                const size_t row = number_of(u, h, r0 + r);
+                float* to = all ? a.out + row * dh : TILED ? part + row * dh : po + (size_t)r * dh;
+                row_again<T>(a, b, h, u.s.first + (int)((r0 + r) / a.rep), u, t0, t1, a.q + row * dh, to, all ? nullptr : TILED ? stat + row : ps + r);
             }
         }
         turn ^= 1u;
@@ -448,7 +499,7 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
         if (++h == KVH) {
             h = 0;
             u.tiles = 0;
-            while (u.tiles == 0 && ++b < a.c.B) u = unit_of(a, b);
+            while (u.tiles == 0 && ++b < a.c.B) u = unit_of(a, b, 0);
             if (b >= a.c.B) return;
         }
     }
@@ -460,8 +511,7 @@ constexpr uint32_t kMergeGroups = 4;
 __global__ void __launch_bounds__(kMergeGroups * 128) attn_few_merge_kernel(const __grid_constant__ AttnCall a, const float* part, const float2* stat, const Part* meta, uint32_t slot_rows) {
     __shared__ float so[kMergeGroups][128];
     __shared__ float2 sml[kMergeGroups];
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    pdl_enter();
     const uint32_t c = blockIdx.x + 1, r = blockIdx.y, d = threadIdx.x, grp = threadIdx.y, dh = a.c.dh;
     const Part p = meta[c];
     if (p.b < 0 || !p.first) return;
@@ -492,37 +542,55 @@ __global__ void __launch_bounds__(kMergeGroups * 128) attn_few_merge_kernel(cons
     a.out[((size_t)(s.q0 + r / a.rep) * a.H + p.h * a.rep + r % a.rep) * dh + d] = L == 0.f ? 0.f : o / L;
 }
 
+template <typename T, int DHP, bool PAIR, bool TILED = false>
+bool ready_kernel() {
+    auto* kernel = attn_few_kernel<T, DHP, PAIR, TILED>;
+    static PerDevice<bool> ready;
+    int dev = -1;
+    if (cudaGetDevice(&dev) == cudaSuccess && ready.get(dev, [=](bool&) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Few<T, DHP, PAIR>::Smem) == cudaSuccess; }))
+        return true;
+    return fail("attention: shared memory attribute: %s", cudaGetErrorString(cudaGetLastError()));
+}
+
 template <typename T, int DHP, bool PAIR>
 bool go(const AttnCall& a, float* scratch, cudaStream_t st) {
     using F = Few<T, DHP, PAIR>;
-    auto* kernel = attn_few_kernel<T, DHP, PAIR>;
-    static PerDevice<bool> ready;
-    int dev = -1;
-    if (cudaGetDevice(&dev) != cudaSuccess || !ready.get(dev, [=](bool&) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)F::Smem) == cudaSuccess; }))
-        return fail("attention: shared memory attribute: %s", cudaGetErrorString(cudaGetLastError()));
+    if (!ready_kernel<T, DHP, PAIR>()) return false;
     const unsigned most = std::min(kFewCtas, (unsigned)device_sm_count() * F::PerSm);
     const unsigned long long tiles = (unsigned long long)a.c.B * a.c.KVH * (((unsigned long long)(a.c.table ? a.c.cap : a.c.total) + kTile - 1) / kTile);
     const unsigned grid = tiles < most ? (unsigned)std::max(tiles, 1ull) : most;
     Part* meta = reinterpret_cast<Part*>(scratch);
     float2* stat = reinterpret_cast<float2*>(meta + kFewCtas);
     float* part = reinterpret_cast<float*>(stat + 2 * kFewCtas * F::Rows);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid); cfg.blockDim = dim3(32 * kWarps); cfg.dynamicSmemBytes = F::Smem; cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at; cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, kernel, a, part, stat, meta);
+    launch_overlapped(attn_few_kernel<T, DHP, PAIR, false>, dim3(grid), dim3(32 * kWarps), F::Smem, st, a, part, stat, meta, 1u);
     note_launch();
     if (!check_launch("attn_few")) return false;
     if (grid == 1) return true;
-    cfg.gridDim = dim3(grid - 1, std::min(F::Rows, a.max_q >= F::Rows ? F::Rows : a.max_q * a.rep)); cfg.blockDim = dim3(128, kMergeGroups); cfg.dynamicSmemBytes = 0;
-    cudaLaunchKernelEx(&cfg, attn_few_merge_kernel, a, (const float*)part, (const float2*)stat, (const Part*)meta, (uint32_t)F::Rows);
+    const unsigned rows = a.max_q >= F::Rows ? F::Rows : std::min(F::Rows, a.max_q * a.rep);
+    launch_overlapped(attn_few_merge_kernel, dim3(grid - 1, rows), dim3(128, kMergeGroups), 0, st, a, part, stat, meta, F::Rows);
     note_launch();
     return check_launch("attn_few_merge");
 }
 
+template <int DHP>
+bool go_tiled(const AttnCall& a, const ChunkPlan& pl, float* scratch, cudaStream_t st) {
+    using F = Few<float, DHP, false>;
+    if (!ready_kernel<float, DHP, false, true>()) return false;
+    const unsigned long long ctas = (unsigned long long)a.c.KVH * pl.splits * pl.slots;
+    if (ctas > 0x7fffffffull) return fail("attention: %llu tiles of query rows", ctas);
+    float* part = scratch;
+    float2* stat = reinterpret_cast<float2*>(part + (size_t)pl.splits * a.c.T * a.H * a.c.dh);
+    launch_overlapped(attn_few_kernel<float, DHP, false, true>, dim3((unsigned)ctas), dim3(32 * kWarps), F::Smem, st, a, part, stat, (Part*)nullptr, pl.splits);
+    note_launch();
+    return check_launch("attn_tiled") && (pl.splits == 1 || launch_attn_merge(a, pl.splits, part, stat, st));
+}
+
 }  // namespace
+
+bool launch_attn_tiled(AttnCall a, const ChunkPlan& pl, float* scratch, cudaStream_t st) {
+    a.tiled = true;
+    return a.c.dh <= 64 ? go_tiled<64>(a, pl, scratch, st) : go_tiled<128>(a, pl, scratch, st);
+}
 
 size_t attn_few_scratch(uint32_t rows, uint32_t dh) {
     const size_t slots = 2 * (size_t)kFewCtas * (rows <= 8 ? 8 : kFewRows);

@@ -1,5 +1,5 @@
 // attn_pages.cu — attention of the new tokens of a batch of sequences over a paged K/V cache, and of a chunk of tokens over a
-// contiguous one, with an optional sliding window and first tokens that stay visible. The simple form: a warp per query row.
+// contiguous one, with an optional sliding window and first tokens that stay visible: the entries, their checks, and which kernel serves what.
 #include "cuda_shim.h"
 #include "attn_pages.h"
 #include "common.cuh"
@@ -7,8 +7,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <cuda_fp16.h>
-#include <math_constants.h>
 
 namespace tmc {
 
@@ -36,48 +34,8 @@ bool kv_batch_from(KvBatch* c, const tm_cuda_kv_pages* kv, unsigned T, unsigned 
 
 namespace {
 
-template <typename T>
-__global__ void __launch_bounds__(128) attn_rows_kernel(const __grid_constant__ AttnCall a) {
-    const KvBatch& c = a.c;
-    const uint32_t lane = threadIdx.x & 31u, id = blockIdx.x * 4u + (threadIdx.x >> 5), t = id / a.H, head = id % a.H;
-    if (t >= c.T) return;
-    const uint32_t b = kv_find_seq(c, t);
-    if (b >= c.B) return;
-    const KvSeq s = kv_seq(c, b);
-    if (s.lost || t < s.q0 || t - s.q0 >= s.n) { note_bad_batch(a.status); return; }
-    if (s.n * a.rep <= a.few) return;
-    const uint32_t dh = c.dh;
-    const int p = s.first + (int)(t - s.q0);
-    const KvSpan span = kv_span(a.mask, p, p);
-    const T* kb = (const T*)c.k + (size_t)(head / a.rep) * c.page * dh;
-    const T* vb = (const T*)c.v + (size_t)(head / a.rep) * c.page * dh;
-    float qr[4], acc[4] = {}, m = -CUDART_INF_F, l = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) qr[i] = lane + 32u * i < dh ? a.q[((size_t)t * a.H + head) * dh + lane + 32u * i] * (a.scale * kLog2e) : 0.f;
-    bool bad = s.bad || s.n > a.max_q;
-    for (uint32_t j = span.a ? 0u : span.b; j < span.e; j = j + 1 == span.a ? span.b : j + 1) {
-        size_t at;
-        if (!kv_row(c, b, j, &at)) { bad = true; continue; }
-        float x = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (lane + 32u * i < dh) x = fmaf(qr[i], (float)kb[at + lane + 32u * i], x);
-#pragma unroll
-        for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-        const float mn = fmaxf(m, x), corr = m == -CUDART_INF_F ? 0.f : exp2f(m - mn), w = x == -CUDART_INF_F ? 0.f : exp2f(x - mn + kUp);
-        l = fmaf(l, corr, w);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (lane + 32u * i < dh) acc[i] = fmaf(acc[i], corr, w * (float)vb[at + lane + 32u * i]);
-        m = mn;
-    }
-    if (bad) { note_bad_batch(a.status); l = CUDART_NAN_F; }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (lane + 32u * i < dh) a.out[((size_t)t * a.H + head) * dh + lane + 32u * i] = l == 0.f ? 0.f : acc[i] / l;
-}
-
-// Which kernels serve a call: sequences with up to `few` rows per K/V head attn_few.cu, those with more (`others`: there may be some) this one.
+// Which kernels serve a call: sequences with up to `few` rows per K/V head attn_few.cu, those with more (`others`: there may be some) attn_chunk.cu, or, over
+// fp32 caches, attn_few.cu again with 16 rows at a time.
 struct Split { uint32_t few; bool others; };
 Split split(unsigned B, unsigned long long rows, unsigned rep) {
     if (rows <= kFewRows) return Split{rows <= 8 ? 8u : kFewRows, false};
@@ -91,11 +49,9 @@ bool launch(AttnCall a, bool half, float* scratch, cudaStream_t st) {
     a.few = sp.few; a.others = sp.others; a.status = device_status_word();
     if (sp.few && !launch_attn_few(a, half, scratch, st)) return false;
     if (!sp.others) return true;
-    if (half) return launch_attn_chunk(a, plan_attn_chunk(a.c.T, a.c.B, a.c.KVH, a.rep, a.few), scratch + few_bytes(sp, a.c.dh) / sizeof(float), st);
-    const unsigned grid = (unsigned)(((size_t)a.c.T * a.H + 3) / 4);
-    attn_rows_kernel<float><<<grid, 128, 0, st>>>(a);
-    note_launch();
-    return check_launch("attention");
+    const ChunkPlan pl = plan_attn_chunk(a.c.T, a.c.B, a.c.KVH, a.rep, a.few, half ? kChunkRows : kFewRows);
+    float* own = scratch + few_bytes(sp, a.c.dh) / sizeof(float);
+    return half ? launch_attn_chunk(a, pl, own, st) : launch_attn_tiled(a, pl, own, st);
 }
 
 }  // namespace
@@ -109,7 +65,9 @@ size_t tm_cuda_attn_paged_scratch(unsigned T, unsigned B, unsigned max_q, unsign
     if (!KVH || !H || H % KVH || !dh || !T) return 16;
     const unsigned rep = H / KVH;
     const Split sp = split(B, (unsigned long long)(max_q && max_q < T ? max_q : T) * rep, rep);
-    const size_t chunk = sp.others ? attn_chunk_scratch(plan_attn_chunk(T, B, KVH, rep, sp.few), T, H, dh) : 0;
+    size_t chunk = 0;
+    if (sp.others)                                              // of either type of cache
+        for (const uint32_t tile : {kChunkRows, kFewRows}) chunk = std::max(chunk, attn_chunk_scratch(plan_attn_chunk(T, B, KVH, rep, sp.few, tile), T, H, dh));
     return std::max<size_t>(16, few_bytes(sp, dh) + chunk);
 }
 size_t tm_cuda_attn_window_scratch(unsigned T, unsigned H, unsigned KVH, unsigned dh) { return tm_cuda_attn_paged_scratch(T, 1, T, H, KVH, dh); }
@@ -125,7 +83,7 @@ bool tm_cuda_attn_paged_dev(const tm_cuda_kv_pages* kv, const float* q, float* s
     if (scratch_bytes < need) return fail("attn_paged: %zu bytes of scratch, %zu are needed", scratch_bytes, need);
     if (!on_library_device("attn_paged")) return false;
     if (!T) return true;
-    return launch(AttnCall{c, kv_mask(window, sinks), q, out, H, H / c.KVH, max_q && max_q < T ? max_q : T, 0, false, scale, nullptr}, kv->kv_half != 0, scratch, (cudaStream_t)stream);
+    return launch(AttnCall{c, kv_mask(window, sinks), q, out, H, H / c.KVH, max_q && max_q < T ? max_q : T, 0, false, scale, nullptr, false}, kv->kv_half != 0, scratch, (cudaStream_t)stream);
 }
 
 bool tm_cuda_attn_window_dev(const float* q, const void* kc, const void* vc, float* scratch, size_t scratch_bytes, float* out, unsigned T,
@@ -143,7 +101,7 @@ bool tm_cuda_attn_window_dev(const float* q, const void* kc, const void* vc, flo
     if (!on_library_device("attn_window")) return false;
     if (!T) return true;
     const KvBatch c{kc, vc, nullptr, nullptr, nullptr, 1, KVH, dh, ctx, 1, 1, T, ctx, pos0 + T, -1};
-    return launch(AttnCall{c, kv_mask(window, sinks), q, out, H, H / KVH, T, 0, false, scale, nullptr}, kv_half != 0, scratch, (cudaStream_t)stream);
+    return launch(AttnCall{c, kv_mask(window, sinks), q, out, H, H / KVH, T, 0, false, scale, nullptr, false}, kv_half != 0, scratch, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -16,17 +16,20 @@ struct AttnCall {
     bool others;                // sequences with more rows are served by another launch of the same call
     float scale;
     int* status;
+    bool tiled;                 // attn_few.cu: rows in tiles (launch_attn_tiled sets it)
 };
 
 // attn_few.cu: sequences with at most 16 query rows per K/V head
-constexpr uint32_t kFewRows = 16, kFewCtas = 296;       // two CTAs on each of 148 SMs
+constexpr uint32_t kChunkRows = 256, kFewRows = 16, kFewCtas = 296;       // two CTAs on each of 148 SMs
 size_t attn_few_scratch(uint32_t rows, uint32_t dh);
 bool launch_attn_few(const AttnCall& a, bool half, float* scratch, cudaStream_t st);
 
-// attn_chunk.cu: sequences with more rows, over fp16 caches
-struct ChunkPlan { uint32_t slots, splits; };           // (sequence, 256 rows) at most; parts that the keys of one are split into
-ChunkPlan plan_attn_chunk(uint32_t T, uint32_t B, uint32_t KVH, uint32_t rep, uint32_t few);
+// Sequences with more rows, in tiles of row_tile: 256 over fp16 caches (attn_chunk.cu), 16 over fp32 ones (attn_few.cu).
+struct ChunkPlan { uint32_t slots, splits; };           // (sequence, tile of rows) at most; parts that the keys of one are split into
+ChunkPlan plan_attn_chunk(uint32_t T, uint32_t B, uint32_t KVH, uint32_t rep, uint32_t few, uint32_t row_tile);
 size_t attn_chunk_scratch(const ChunkPlan& pl, uint32_t T, uint32_t H, uint32_t dh);
 bool launch_attn_chunk(const AttnCall& a, const ChunkPlan& pl, float* scratch, cudaStream_t st);
+bool launch_attn_tiled(AttnCall a, const ChunkPlan& pl, float* scratch, cudaStream_t st);
+bool launch_attn_merge(const AttnCall& a, uint32_t splits, const float* part, const float2* stat, cudaStream_t st);
 
 }  // namespace tmc

@@ -8,6 +8,7 @@
 #include "cuda_shim.h"
 #include "common.cuh"
 #include "kv_pages.cuh"
+#include "pdl.cuh"
 #include "state.h"
 
 #include <cuda_fp16.h>
@@ -27,21 +28,24 @@ template <typename T>
 __global__ void __launch_bounds__(256) kv_append_kernel(KvBatch c, const float* qkv, float* q, uint32_t H, const float2* rope, uint32_t rope_rows,
                                                         int* status) {
     const uint32_t t = blockIdx.x, dh = c.dh, KVH = c.KVH, half = dh / 2, per = dh / 8, turned = (H + KVH) * per;
-    const uint32_t e = blockIdx.y * blockDim.x + threadIdx.x;
-    const uint32_t b = kv_find_seq(c, t);
-    if (b >= c.B) return;                                       // behind the last sequence
-    const KvSeq s = kv_seq(c, b);
-    const int pos = s.first + (int)(t - s.q0);
-    if (s.lost || s.bad || t < s.q0 || t - s.q0 >= s.n || (rope && pos >= (int)rope_rows)) { note_bad_batch(status); return; }
-    if (pos < 0) return;
+    const uint32_t e = blockIdx.y * blockDim.x + threadIdx.x, i = 4 * (e - turned), h = e / per, j = 4 * (e % per);
     const float* row = qkv + (size_t)t * (H + 2 * KVH) * dh;
+    const bool turns = e < turned, value = !turns && i < KVH * dh;
+    pdl_enter();
+    float4 u = make_float4(0.f, 0.f, 0.f, 0.f), w = u;          // on their way while the sequence is looked for
+    if (turns) { u = *reinterpret_cast<const float4*>(row + (size_t)h * dh + j); w = *reinterpret_cast<const float4*>(row + (size_t)h * dh + j + half); }
+    else if (value) u = *reinterpret_cast<const float4*>(row + (size_t)(H + KVH) * dh + i);
+    if (t == 0 && blockIdx.y == 0) kv_note_lost(c, status);
+    uint32_t b;
+    KvSeq s;
+    if (!kv_find_seq(c, t, &b, &s)) return;                     // behind the last sequence
+    const int pos = s.first + (int)(t - s.q0);
+    if (s.bad || (rope && pos >= (int)rope_rows)) { note_bad_batch(status); return; }
+    if (pos < 0) return;
     size_t at;
     const bool page = kv_row(c, b, (uint32_t)pos, &at);
     if (!page) note_bad_batch(status);
-    if (e < turned) {
-        const uint32_t h = e / per, j = 4 * (e % per);
-        const float* x = row + (size_t)h * dh + j;
-        const float4 u = *reinterpret_cast<const float4*>(x), w = *reinterpret_cast<const float4*>(x + half);
+    if (turns) {
         float4 lo = u, hi = w;
         if (rope) {
             const float4* cs = reinterpret_cast<const float4*>(rope + (size_t)pos * half + j);
@@ -56,9 +60,8 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvBatch c, const float* 
             T* o = (T*)const_cast<void*>(c.k) + at + (size_t)(h - H) * c.page * dh + j;
             store4(o, lo); store4(o + half, hi);
         }
-    } else if (const uint32_t i = 4 * (e - turned); i < KVH * dh && page) {
-        const uint32_t h = i / dh, l = i % dh;
-        store4((T*)const_cast<void*>(c.v) + at + (size_t)h * c.page * dh + l, *reinterpret_cast<const float4*>(row + (size_t)(H + KVH) * dh + i));
+    } else if (value && page) {
+        store4((T*)const_cast<void*>(c.v) + at + (size_t)(i / dh) * c.page * dh + i % dh, u);
     }
 }
 
@@ -78,8 +81,8 @@ extern "C" bool tm_cuda_kv_append_paged_dev(const tm_cuda_kv_pages* kv, const fl
     if (!on_library_device("kv_append_paged")) return false;
     if (!T) return true;
     const dim3 grid(T, ((H + c.KVH) * (c.dh / 8) + c.KVH * c.dh / 4 + 255) / 256);
-    if (kv->kv_half) kv_append_kernel<__half><<<grid, 256, 0, (cudaStream_t)stream>>>(c, qkv, q, H, (const float2*)rope, rope_rows, device_status_word());
-    else kv_append_kernel<float><<<grid, 256, 0, (cudaStream_t)stream>>>(c, qkv, q, H, (const float2*)rope, rope_rows, device_status_word());
+    launch_overlapped(kv->kv_half ? kv_append_kernel<__half> : kv_append_kernel<float>, grid, dim3(256), 0, (cudaStream_t)stream, c, qkv, q, H, (const float2*)rope,
+                      rope_rows, device_status_word());
     note_launch();
     return check_launch("kv_append_paged");
 }

@@ -68,12 +68,29 @@ TM_HD bool kv_row(const KvBatch& c, uint32_t b, uint32_t pos, size_t* at) {
 __device__ __forceinline__ void note_bad_batch(int* status) {
     if (status) *(volatile int*)status = kStatusBatch;
 }
-// The sequence that token t belongs to, found by a whole warp: as many q_begin[1..B] as are at most t. B: none.
-__device__ __forceinline__ uint32_t kv_find_seq(const KvBatch& c, uint32_t t) {
-    if (!c.table) return 0;
-    uint32_t before = 0;
-    for (uint32_t i = threadIdx.x & 31u; i < c.B; i += 32) before += c.q_begin[i + 1] <= (int)t;
-    return __reduce_add_sync(0xffffffffu, before);
+// The sequence that token t belongs to, found by a whole warp: a lane reads all there is to know of a sequence, so that one trip to memory
+// says which it is and what it is. false: none.
+__device__ __forceinline__ bool kv_find_seq(const KvBatch& c, uint32_t t, uint32_t* b, KvSeq* s) {
+    if (!c.table) { *b = 0; *s = kv_seq(c, 0); return true; }
+    const uint32_t lane = threadIdx.x & 31u;
+    for (uint32_t i0 = 0; i0 < c.B; i0 += 32) {
+        KvSeq x{};
+        if (i0 + lane < c.B) x = kv_seq(c, i0 + lane);
+        const uint32_t here = __ballot_sync(0xffffffffu, t - x.q0 < x.n);
+        if (!here) continue;
+        const int at = __ffs((int)here) - 1;
+        *b = i0 + (uint32_t)at;
+        s->q0 = __shfl_sync(0xffffffffu, x.q0, at); s->n = __shfl_sync(0xffffffffu, x.n, at); s->len = __shfl_sync(0xffffffffu, x.len, at);
+        s->first = (int)s->len - (int)s->n; s->lost = false; s->bad = __shfl_sync(0xffffffffu, (int)x.bad, at) != 0;
+        return true;
+    }
+    return false;
+}
+// A range of rows that is none, noted by whoever walks all sequences anyway
+__device__ __forceinline__ void kv_note_lost(const KvBatch& c, int* status) {
+    if (!c.table) return;
+    for (uint32_t i = threadIdx.x; i < c.B; i += blockDim.x)
+        if (kv_seq(c, i).lost) note_bad_batch(status);
 }
 #endif
 

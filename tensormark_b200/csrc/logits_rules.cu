@@ -10,6 +10,7 @@
 #include "cuda_shim.h"
 #include "common.cuh"
 #include "kv_pages.cuh"
+#include "pdl.cuh"
 #include "state.h"
 
 #include <math_constants.h>
@@ -17,8 +18,7 @@
 namespace tmc {
 namespace {
 
-constexpr uint32_t kSlice = 4096;           // entries of a CTA: 16 KB of counts and as much for the biases, six CTAs per SM
-constexpr uint32_t kThreads = 256;
+constexpr uint32_t kThreads = 256, kWide = 4;                // threads of a CTA, logits of a load
 constexpr uint32_t kPast = 1u << 31;        // occurs in the prompt; below it the number of times among the generated tokens
 
 struct Rules {
@@ -29,45 +29,108 @@ struct Rules {
     uint32_t tokens_ld, bias_ld, mask_ld;
 };
 
+// ITEMS loads per thread: a CTA's slice is ITEMS * 1024 logits. VEC: x and out rows lie alike against 16 bytes, and slices begin on
+// such a boundary; else the same places are read one by one.
+template <uint32_t ITEMS, bool VEC>
 __global__ void __launch_bounds__(kThreads) logits_rules_kernel(const float* x, size_t ldx, float* out, size_t ldo, uint32_t V, Rules r) {
-    __shared__ uint32_t count[kSlice];
-    __shared__ uint32_t bias_at[kSlice];    // 1 + the place in the row's list of biases, 0: none
-    const uint32_t b = blockIdx.y, lo = blockIdx.x * kSlice, n = min(kSlice, V - lo);
+    constexpr uint32_t SLICE = ITEMS * kThreads * kWide;
+    __shared__ __align__(16) uint32_t count[SLICE];
+    __shared__ __align__(16) uint32_t bias_at[SLICE];       // 1 + the place in the row's list of biases, 0: none
+    __shared__ uint32_t words[SLICE / 32 + 1];
+    const uint32_t b = blockIdx.y, tid = threadIdx.x;
+    const float* xr = x + b * ldx;
+    float* o = out + b * ldo;
+    // logits [lo, lo + SLICE), of which those from 0 to V exist
+    const int lo = (int)(blockIdx.x * SLICE) - (VEC ? (int)((uintptr_t)xr / sizeof(float) & (kWide - 1)) : 0);
+    pdl_enter();
+    // the logits, the mask and the rules of the row are on their way while the lists are counted
+    float v[ITEMS][kWide];
+#pragma unroll
+    for (uint32_t k = 0; k < ITEMS; ++k) {
+        const int i = lo + (int)((k * kThreads + tid) * kWide);
+        if (VEC && i >= 0 && i + (int)kWide <= (int)V) {
+            const float4 f = *reinterpret_cast<const float4*>(xr + i);
+            v[k][0] = f.x; v[k][1] = f.y; v[k][2] = f.z; v[k][3] = f.w;
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < kWide; ++e) v[k][e] = (uint32_t)(i + (int)e) < V ? xr[i + (int)e] : 0.f;
+        }
+    }
+    const int w0 = lo >> 5, most = (int)((V + 31) / 32);
+    if (r.mask)
+        for (uint32_t i = tid; i <= SLICE / 32; i += kThreads) words[i] = (uint32_t)(w0 + (int)i) < (uint32_t)most ? r.mask[(size_t)b * r.mask_ld + (uint32_t)(w0 + (int)i)] : 0u;
     const uint32_t listed = r.tokens ? (uint32_t)min(max(r.n_tokens[b], 0), (int)r.tokens_ld) : 0u;
     const uint32_t biases = r.bias ? (uint32_t)min(max(r.n_bias ? r.n_bias[b] : (int)r.bias_ld, 0), (int)r.bias_ld) : 0u;
     const int prompt = r.n_prompt ? r.n_prompt[b] : 0;
-    if (listed) for (uint32_t i = threadIdx.x; i < n; i += kThreads) count[i] = 0;
-    if (biases) for (uint32_t i = threadIdx.x; i < n; i += kThreads) bias_at[i] = 0;
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < listed; i += kThreads) {
-        const uint32_t at = (uint32_t)r.tokens[(size_t)b * r.tokens_ld + i] - lo;     // ids outside the vocabulary are in no slice
-        if (at < n) {
-            if ((int)i < prompt) atomicOr(&count[at], kPast);
-            else atomicAdd(&count[at], 1u);
-        }
-    }
-    for (uint32_t i = threadIdx.x; i < biases; i += kThreads) {
-        const uint32_t at = (uint32_t)r.bias_ids[(size_t)b * r.bias_ld + i] - lo;
-        if (at < n) atomicMax(&bias_at[at], i + 1);                                   // of an id that is listed twice the last one counts
-    }
-    __syncthreads();
     const float repeat = r.repeat ? r.repeat[b] : 1.f, presence = r.presence ? r.presence[b] : 0.f, frequency = r.frequency ? r.frequency[b] : 0.f;
-    const float* xr = x + b * ldx + lo;
-    float* o = out + b * ldo + lo;
-    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-        float v = xr[i];
-        if (listed) {
-            const uint32_t c = count[i];
-            if (c) {
-                v = v > 0.f ? v / repeat : v * repeat;
-                const float made = (float)(c & ~kPast);
-                if (made > 0.f) v -= fmaf(frequency, made, presence);
+    if (listed) for (uint32_t i = tid; i < SLICE / 4; i += kThreads) reinterpret_cast<uint4*>(count)[i] = make_uint4(0, 0, 0, 0);
+    if (biases) for (uint32_t i = tid; i < SLICE / 4; i += kThreads) reinterpret_cast<uint4*>(bias_at)[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    const int* tokens = r.tokens + (size_t)b * r.tokens_ld;
+    constexpr uint32_t AHEAD = 4;
+    for (uint32_t i0 = tid; i0 < listed; i0 += AHEAD * kThreads) {
+        int id[AHEAD];
+#pragma unroll
+        for (uint32_t k = 0; k < AHEAD; ++k) id[k] = i0 + k * kThreads < listed ? tokens[i0 + k * kThreads] : -1;
+#pragma unroll
+        for (uint32_t k = 0; k < AHEAD; ++k) {
+            const uint32_t at = (uint32_t)(id[k] - lo);
+            if ((uint32_t)id[k] < V && at < SLICE) {        // an id outside the vocabulary is in no slice
+                if ((int)(i0 + k * kThreads) < prompt) atomicOr(&count[at], kPast);
+                else atomicAdd(&count[at], 1u);
             }
         }
-        if (biases && bias_at[i]) v += r.bias[(size_t)b * r.bias_ld + bias_at[i] - 1];
-        if (r.mask && !(r.mask[(size_t)b * r.mask_ld + ((lo + i) >> 5)] >> ((lo + i) & 31u) & 1u)) v = -CUDART_INF_F;
-        o[i] = v;
     }
+    for (uint32_t i = tid; i < biases; i += kThreads) {
+        const int id = r.bias_ids[(size_t)b * r.bias_ld + i];
+        const uint32_t at = (uint32_t)(id - lo);
+        if ((uint32_t)id < V && at < SLICE) atomicMax(&bias_at[at], i + 1);            // of an id that is listed twice the last one counts
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t k = 0; k < ITEMS; ++k) {
+        const uint32_t at = (k * kThreads + tid) * kWide;
+        const int i = lo + (int)at;
+        if (listed) {
+            const uint4 c4 = *reinterpret_cast<const uint4*>(count + at);
+            const uint32_t c[kWide] = {c4.x, c4.y, c4.z, c4.w};
+#pragma unroll
+            for (uint32_t e = 0; e < kWide; ++e)
+                if (c[e]) {
+                    v[k][e] = v[k][e] > 0.f ? v[k][e] / repeat : v[k][e] * repeat;
+                    const float made = (float)(c[e] & ~kPast);
+                    if (made > 0.f) v[k][e] -= fmaf(frequency, made, presence);
+                }
+        }
+        if (biases) {
+            const uint4 c4 = *reinterpret_cast<const uint4*>(bias_at + at);
+            const uint32_t c[kWide] = {c4.x, c4.y, c4.z, c4.w};
+#pragma unroll
+            for (uint32_t e = 0; e < kWide; ++e)
+                if (c[e]) v[k][e] += r.bias[(size_t)b * r.bias_ld + c[e] - 1];
+        }
+        if (r.mask) {
+#pragma unroll
+            for (uint32_t e = 0; e < kWide; ++e) {
+                const uint32_t bit = (uint32_t)(i + (int)e - w0 * 32);
+                if (!(words[bit >> 5] >> (bit & 31u) & 1u)) v[k][e] = -CUDART_INF_F;
+            }
+        }
+        if (VEC && i >= 0 && i + (int)kWide <= (int)V) *reinterpret_cast<float4*>(o + i) = make_float4(v[k][0], v[k][1], v[k][2], v[k][3]);
+        else {
+#pragma unroll
+            for (uint32_t e = 0; e < kWide; ++e)
+                if ((uint32_t)(i + (int)e) < V) o[i + (int)e] = v[k][e];
+        }
+    }
+}
+
+template <uint32_t ITEMS>
+void go(const float* x, size_t ldx, float* out, size_t ldo, unsigned B, unsigned V, const Rules& r, cudaStream_t st) {
+    constexpr uint32_t SLICE = ITEMS * kThreads * kWide;
+    const bool vec = (uintptr_t)x % 16 == (uintptr_t)out % 16 && (B == 1 || ldx % kWide == ldo % kWide);
+    const dim3 grid((unsigned)(((unsigned long long)V + (vec ? kWide - 1 : 0) + SLICE - 1) / SLICE), B);
+    launch_overlapped(vec ? logits_rules_kernel<ITEMS, true> : logits_rules_kernel<ITEMS, false>, grid, dim3(kThreads), 0, st, x, ldx, out, ldo, V, r);
 }
 
 }  // namespace
@@ -78,7 +141,7 @@ using namespace tmc;
 extern "C" bool tm_cuda_logits_rules_dev(const float* x, size_t ldx, float* out, size_t ldo, unsigned B, unsigned V,
                                          const tm_cuda_logit_rules* rules, void* stream) {
     if (!x || !out || !rules) return fail("logits_rules: null pointer");
-    if (!V || V > 0x7fffffffu || B > 65535u || ldx < V || ldo < V) return fail("logits_rules: %u rows of %u logits in strides of %zu and %zu", B, V, ldx, ldo);
+    if (!V || V > 0x7fff0000u || B > 65535u || ldx < V || ldo < V) return fail("logits_rules: %u rows of %u logits in strides of %zu and %zu", B, V, ldx, ldo);
     const tm_cuda_logit_rules& r = *rules;
     if (r.tokens && (!r.n_tokens || !r.tokens_ld || r.tokens_ld > 0x7fffffffu)) return fail("logits_rules: a token list without lengths or stride");
     if (!r.tokens && (r.repeat || r.presence || r.frequency)) return fail("logits_rules: penalties without a token list");
@@ -87,7 +150,9 @@ extern "C" bool tm_cuda_logits_rules_dev(const float* x, size_t ldx, float* out,
     if (!on_library_device("logits_rules")) return false;
     if (!B) return true;
     const Rules k{r.tokens, r.n_tokens, r.n_prompt, r.repeat, r.presence, r.frequency, r.bias_ids, r.bias, r.n_bias, r.mask, r.tokens_ld, r.bias_ld, r.mask_ld};
-    logits_rules_kernel<<<dim3(V / kSlice + (V % kSlice != 0), B), kThreads, 0, (cudaStream_t)stream>>>(x, ldx, out, ldo, V, k);
+    // Slices of 4096 read the lists a quarter as often, slices of 1024 spread a small batch over the SMs.
+    if ((unsigned long long)B * V >= 148ull * 4096) go<4>(x, ldx, out, ldo, B, V, k, (cudaStream_t)stream);
+    else go<1>(x, ldx, out, ldo, B, V, k, (cudaStream_t)stream);
     note_launch();
     return check_launch("logits_rules");
 }
