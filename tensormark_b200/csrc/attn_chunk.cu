@@ -148,7 +148,7 @@ __device__ __forceinline__ bool wait_for(uint64_t& bar, uint32_t parity, volatil
 struct Bars { uint64_t full[6], empty[6], ready[2], done[2]; };
 
 template <int DHP>
-__global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_constant__ AttnCall a, uint32_t splits, float* part, float2* stat) {
+__global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_constant__ AttnCall a, uint32_t splits) {
     using C = Chunk<DHP>;
     constexpr uint32_t NBUF = C::Buffers;
     extern __shared__ uint8_t smem_dyn[];
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
     pdl_enter();
 
     // ---- which sequence, and which of its row tiles: counted from the last one (the longest of a prompt) ----
-    const uint32_t at_once = a.c.KVH * splits, slot = (gridDim.x - 1 - blockIdx.x) / at_once, h = blockIdx.x % at_once % a.c.KVH, split = blockIdx.x % at_once / a.c.KVH;
+    const uint32_t unit = (gridDim.x - 1 - blockIdx.x) / splits, slot = unit / a.c.KVH, h = unit % a.c.KVH, split = blockIdx.x % splits;
     auto slots_of = [&](uint32_t b, bool note) {
         const KvSeq s = kv_seq(a.c, b);
         if (s.lost && note) note_bad_batch(a.status);
@@ -204,7 +204,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
     kt.set(kv_span(a.mask, p_first, p_last), bad);
     const uint32_t t0 = (uint32_t)((unsigned long long)kt.tiles * split / splits), t1 = (uint32_t)((unsigned long long)kt.tiles * (split + 1) / splits), n = t1 - t0;
 
+    auto number_of = [&](uint32_t i) {                                   // of a row in q and out
+        const uint32_t tok = (uint32_t)(place[i] - s.first);
+        return (size_t)(s.q0 + tok) * a.H + h * a.rep + (row0 + i - tok * a.rep);
+    };
     const uint32_t region = (smem_u32(smem_dyn) + 1023u) & ~1023u, ring = region + 4 * C::Tile;
+    // where the results go in the end: 16 bytes more than a row, so that threads with a row each store without conflicts
+    constexpr uint32_t PITCH = DHP * 4 + 16;
+    const uint32_t stats = region + 2 * kRows * PITCH;
+    static_assert(2 * kRows * (PITCH + 8) <= (4 + C::Buffers) * C::Tile, "the results fit");
     if (tid == 0) {
         for (uint32_t i = 0; i < NBUF; ++i) { mbar_init(smem_u32(&bars.full[i]), 96); mbar_init(smem_u32(&bars.empty[i]), 1); }
         for (uint32_t i = 0; i < 2; ++i) { mbar_init(smem_u32(&bars.ready[i]), 4); mbar_init(smem_u32(&bars.done[i]), 1); }
@@ -323,10 +331,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const uint32_t w = (warp - 4) >> 2, r = (warp & 3u) * 32 + lane, row = w * kRows + r;
         if (w < tiles2) {
-            auto number_of = [&](uint32_t i) {                           // of the row in q and out
-                const uint32_t tok = (uint32_t)(place[i] - s.first);
-                return (size_t)(s.q0 + tok) * a.H + h * a.rep + (row0 + i - tok * a.rep);
-            };
             int p_min, lo_max;                                           // the least that a row of the warp sees ahead and behind
             {
                 const bool is = row < rows;
@@ -487,27 +491,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
 #pragma unroll
             for (uint32_t d = 0; d < DHP; ++d) finite = finite && fabsf(o[d]) < CUDART_INF_F;
             if (!ok || bad) l = CUDART_NAN_F;
-            const bool is = place[row] != kNoRow;
-            const uint32_t again = __ballot_sync(0xffffffffu, is && ok && !bad && !finite);
+            const uint32_t again = __ballot_sync(0xffffffffu, place[row] != kNoRow && ok && !bad && !finite);
             if (lane == 0) odd[w * 4 + (warp & 3u)] = again;
-            // out: through shared memory (q's, which no product reads any more), so that the stores are whole lines
-            const float inv = splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
-            const uint32_t stage = region + w * 2 * C::Tile;
+            // The rows, unnormalised, and their statistics in shared memory, where q and the ring were: no product reads them any more once
+            // both row tiles are here.
+            asm volatile("bar.sync 1, %0;" ::"r"(tiles2 * 128u) : "memory");
 #pragma unroll
-            for (uint32_t c = 0; c < LR; ++c)
-                asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(stage + r * (DHP * 4) + ((c ^ (r % LR)) << 4)),
-                             "f"(o[4 * c] * inv), "f"(o[4 * c + 1] * inv), "f"(o[4 * c + 2] * inv), "f"(o[4 * c + 3] * inv) : "memory");
-            __syncwarp();
-            const size_t shift = splits > 1 ? (size_t)split * a.c.T * a.H : 0;
-            float* const out = splits > 1 ? part : a.out;
-            if (is && splits > 1) stat[shift + number_of(row)] = make_float2(m, l);
-#pragma unroll 8
-            for (uint32_t i = 0; i < 32; i += RT) {
-                const uint32_t rr = first_row + i + lane / LR, rq = rr % kRows;
-                float4 f;
-                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(stage + rq * (DHP * 4) + ((piece ^ (rq % LR)) << 4)) : "memory");
-                if (rr < rows && 4 * piece < dh) *reinterpret_cast<float4*>(out + (shift + number_of(rr)) * dh + 4 * piece) = f;
-            }
+            for (uint32_t d = 0; d < DHP; d += 4)
+                asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(region + row * PITCH + d * 4), "f"(o[d]), "f"(o[d + 1]), "f"(o[d + 2]), "f"(o[d + 3]) : "memory");
+            asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(stats + row * 8), "f"(m), "f"(l) : "memory");
         }
     }
     if (!ok) { if (a.status) *(volatile int*)a.status = 1; }
@@ -523,86 +515,78 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols) : "memory");
     }
     // ---- rows that are computed again, or whose pages were not all there ----
+    float* const rows_at = reinterpret_cast<float*>(smem_dyn + (region - smem_u32(smem_dyn)));
+    float2* const stats_at = reinterpret_cast<float2*>(smem_dyn + (stats - smem_u32(smem_dyn)));
     if (warp >= 4)
         for (uint32_t i = warp - 4; i < rows; i += 8) {
-            if (!bad_page && !(odd[i >> 5] >> (i & 31u) & 1u)) continue;
-            const uint32_t gi = row0 + i, tok = gi / a.rep;
-            const size_t at = (size_t)(s.q0 + tok) * a.H + h * a.rep + gi % a.rep, to = splits > 1 ? (size_t)split * a.c.T * a.H + at : at;
-            float* out = (splits > 1 ? part : a.out) + to * dh;
-            if (bad_page) {
-                for (uint32_t d = lane; d < dh; d += 32) out[d] = CUDART_NAN_F;
-                if (splits > 1 && lane == 0) stat[to] = make_float2(0.f, CUDART_NAN_F);
-            } else {
-                row_again<__half>(a, b, h, s.first + (int)tok, kt, t0, t1, a.q + at * dh, out, splits > 1 ? stat + to : nullptr);
+            if (bad_page || gone) { if (lane == 0) stats_at[i].y = CUDART_NAN_F; }
+            else if (odd[i >> 5] >> (i & 31u) & 1u) row_again<__half>(a, b, h, place[i], kt, t0, t1, a.q + number_of(i) * dh, rows_at + i * (PITCH / 4), stats_at + i);
+        }
+    // ---- the parts of the cluster's CTAs together: each takes every splits-th turn of a warp, whole lines at a time ----
+    if (splits > 1) cluster_sync(); else __syncthreads();
+    constexpr uint32_t LR = DHP / 4, RT = 32 / LR;                       // lanes of a row, rows of a turn
+    const uint32_t piece = lane % LR;
+    if (warp >= 4) {
+        auto finish = [&](uint32_t rr, float4 y, float L) {
+            const float inv = L == 0.f ? 0.f : 1.f / L;
+            if (rr < rows && 4 * piece < dh)
+                *reinterpret_cast<float4*>(a.out + number_of(rr) * dh + 4 * piece) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+        };
+        if (splits == 1) {
+#pragma unroll 4
+            for (uint32_t i = (warp - 4) * RT; i < rows; i += 8 * RT) {
+                const uint32_t rr = i + lane / LR;
+                finish(rr, *reinterpret_cast<const float4*>(rows_at + rr * (PITCH / 4) + piece * 4), stats_at[rr].y);
+            }
+        } else {
+            for (uint32_t i = ((warp - 4) * splits + split) * RT; i < rows; i += 8 * splits * RT) {
+                const uint32_t rr = i + lane / LR;
+                float M = -CUDART_INF_F, L = 0.f;
+                float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+                for (uint32_t k = 0; k < splits; k += 2) {               // a power of two, so two at a time
+                    const float2 m0 = ld_cta2(map_cta(stats + rr * 8, k)), m1 = ld_cta2(map_cta(stats + rr * 8, k + 1));
+                    const float4 x0 = ld_cta4(map_cta(region + rr * PITCH + piece * 16, k)), x1 = ld_cta4(map_cta(region + rr * PITCH + piece * 16, k + 1));
+                    const float mn = fmaxf(M, fmaxf(m0.x, m1.x)), base = mn == -CUDART_INF_F ? 0.f : mn, f = pow2(M - base), f0 = pow2(m0.x - base), f1 = pow2(m1.x - base);
+                    L = fmaf(L, f, fmaf(f0, m0.y, f1 * m1.y));
+                    y.x = fmaf(y.x, f, fmaf(f0, x0.x, f1 * x1.x)); y.y = fmaf(y.y, f, fmaf(f0, x0.y, f1 * x1.y));
+                    y.z = fmaf(y.z, f, fmaf(f0, x0.z, f1 * x1.z)); y.w = fmaf(y.w, f, fmaf(f0, x0.w, f1 * x1.w));
+                    M = mn;
+                }
+                finish(rr, y, L);
             }
         }
-}
-
-// A warp per row: its parts, weighted by their maxima.
-__global__ void __launch_bounds__(256) attn_chunk_merge_kernel(const __grid_constant__ AttnCall a, uint32_t splits, const float* part, const float2* stat) {
-    pdl_enter();
-    const uint32_t lane = threadIdx.x & 31u, dh = a.c.dh;
-    const size_t rows = (size_t)a.c.T * a.H, row = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (row >= rows) return;
-    uint32_t b;
-    KvSeq s;
-    if (!kv_find_seq(a.c, (uint32_t)(row / a.H), &b, &s) || s.n * a.rep <= a.few) return;
-    float M = -CUDART_INF_F, L = 0.f;
-    for (uint32_t i = 0; i < splits; ++i) M = fmaxf(M, stat[i * rows + row].x);
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (uint32_t i = 0; i < splits; ++i) {
-        const float2 ml = stat[i * rows + row];
-        const float w = ml.x == -CUDART_INF_F ? 0.f : pow2(ml.x - M);
-        L = fmaf(w, ml.y, L);
-        if (4 * lane < dh) {
-            const float4 x = *reinterpret_cast<const float4*>(part + (i * rows + row) * dh + 4 * lane);
-            o.x = fmaf(w, x.x, o.x); o.y = fmaf(w, x.y, o.y); o.z = fmaf(w, x.z, o.z); o.w = fmaf(w, x.w, o.w);
-        }
     }
-    const float by = L == 0.f ? 0.f : 1.f / L;
-    if (4 * lane < dh) *reinterpret_cast<float4*>(a.out + row * dh + 4 * lane) = make_float4(o.x * by, o.y * by, o.z * by, o.w * by);
+    if (splits > 1) cluster_sync();                                      // nobody leaves while its shared memory is read
 }
 
 template <int DHP>
-bool go(const AttnCall& a, const ChunkPlan& pl, float* scratch, cudaStream_t st) {
+bool go(const AttnCall& a, const ChunkPlan& pl, cudaStream_t st) {
     auto* kernel = attn_chunk_kernel<DHP>;
     static PerDevice<bool> ready;
     int dev = -1;
     if (cudaGetDevice(&dev) != cudaSuccess || !ready.get(dev, [=](bool&) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Chunk<DHP>::Smem) == cudaSuccess; }))
         return fail("attention: shared memory attribute: %s", cudaGetErrorString(cudaGetLastError()));
-    const unsigned long long ctas = (unsigned long long)a.c.KVH * pl.splits * pl.slots;
-    if (ctas > 0x7fffffffull) return fail("attention: %llu tiles of query rows", ctas);
-    const size_t rows = (size_t)a.c.T * a.H;
-    float* part = scratch;
-    float2* stat = reinterpret_cast<float2*>(part + pl.splits * rows * a.c.dh);
-    launch_overlapped(kernel, dim3((unsigned)ctas), dim3(kThreads), Chunk<DHP>::Smem, st, a, pl.splits, part, stat);
+    const unsigned long long units = (unsigned long long)a.c.KVH * pl.slots;
+    if (units * pl.splits > 0x7fffffffull) return fail("attention: %llu tiles of query rows", units);
+    if (!launch_units(kernel, (unsigned)units, pl.splits, kThreads, Chunk<DHP>::Smem, st, a, pl.splits)) return false;
     note_launch();
-    if (!check_launch("attn_chunk")) return false;
-    return pl.splits == 1 || launch_attn_merge(a, pl.splits, part, stat, st);
+    return check_launch("attn_chunk");
 }
 
 }  // namespace
-
-bool launch_attn_merge(const AttnCall& a, uint32_t splits, const float* part, const float2* stat, cudaStream_t st) {
-    launch_overlapped(attn_chunk_merge_kernel, dim3((unsigned)(((size_t)a.c.T * a.H + 7) / 8)), dim3(256), 0, st, a, splits, part, stat);
-    note_launch();
-    return check_launch("attn_chunk_merge");
-}
 
 ChunkPlan plan_attn_chunk(uint32_t T, uint32_t B, uint32_t KVH, uint32_t rep, uint32_t few, uint32_t row_tile) {
     const unsigned long long rows = (unsigned long long)T * rep, least = (rows + row_tile - 1) / row_tile;
     ChunkPlan pl;
     pl.slots = (uint32_t)(rows / row_tile + std::min<unsigned long long>(B, rows / (few + 1ull)));
-    pl.splits = (uint32_t)std::max<unsigned long long>(1, std::min<unsigned long long>(148 / (least * KVH), 16));
+    pl.splits = 1;
+    while (pl.splits < 8 && 2 * pl.splits * least * KVH <= 148) pl.splits *= 2;
     return pl;
 }
 
-size_t attn_chunk_scratch(const ChunkPlan& pl, uint32_t T, uint32_t H, uint32_t dh) {
-    return pl.splits == 1 ? 0 : (size_t)pl.splits * T * H * (dh * sizeof(float) + sizeof(float2));
-}
-
-bool launch_attn_chunk(const AttnCall& a, const ChunkPlan& pl, float* scratch, cudaStream_t st) {
-    return a.c.dh <= 64 ? go<64>(a, pl, scratch, st) : go<128>(a, pl, scratch, st);
+bool launch_attn_chunk(const AttnCall& a, const ChunkPlan& pl, cudaStream_t st) {
+    return a.c.dh <= 64 ? go<64>(a, pl, st) : go<128>(a, pl, st);
 }
 
 }  // namespace tmc

@@ -28,6 +28,7 @@ namespace tmc {
 namespace {
 
 constexpr uint32_t kWarps = 4, kTile = 64, kStep = 16;      // keys of a tile; of a warp's share of it
+constexpr uint32_t kClusterTiles = 6;                       // one launch may walk so many tiles more than two would
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -95,9 +96,9 @@ template <typename T, int DHP, bool PAIR> struct Few {
     static constexpr uint32_t PerSm = Smem <= 114688 ? 2 : 1;
 };
 
-// TILED: sequences with more rows than `few`, 16 rows of one per CTA and a share of its keys, `splits` shares; the parts go to part and
-// stat by the number of the row. Else the stretches of the list.
-template <typename T, int DHP, bool PAIR, bool TILED>
+// LIST: the stretches of the list. Else a unit per cluster of `splits` CTAs, which share its keys and merge through distributed shared
+// memory: the rows of a sequence and K/V head, or (a.tiled) 16 of them.
+template <typename T, int DHP, bool PAIR, bool LIST>
 __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_few_kernel(const __grid_constant__ AttnCall a, float* part, float2* stat, Part* meta, uint32_t splits) {
     using F = Few<T, DHP, PAIR>;
     constexpr bool kHalf = sizeof(T) == 2;
@@ -108,41 +109,49 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
     __shared__ uint32_t at_b, at_h, at_t;
     __shared__ float sm_m[kWarps][ROWS], sm_l[kWarps][ROWS];
     __shared__ int sm_bad[2];
+    __shared__ float2 cta_ml[ROWS];                         // what a cluster's CTAs merge: maxima and sums; the outputs lie in the ring
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g = lane >> 2, t4 = lane & 3u;
     pdl_enter();
     const uint32_t dh = a.c.dh, KVH = a.c.KVH;
 
     // ---- this CTA's stretch of the list ----
     unsigned long long x0, x1, total;
-    uint32_t r0 = 0;                                        // TILED: its first row
+    uint32_t r0 = 0;                                        // a.tiled: the unit's first row
+    const uint32_t split = LIST ? 0u : blockIdx.x % splits;
     Unit u0;
-    if constexpr (TILED) {
-        const uint32_t at_once = KVH * splits, slot = (gridDim.x - 1 - blockIdx.x) / at_once, split = blockIdx.x % at_once / KVH;
-        if (tid == 0) { at_b = a.c.B; at_h = blockIdx.x % at_once % KVH; sm_bad[0] = sm_bad[1] = 0; }
-        const uint32_t per = (a.c.B + blockDim.x - 1) / blockDim.x, b0 = min(a.c.B, tid * per), b1 = min(a.c.B, b0 + per);
-        uint32_t mine = 0;
-        for (uint32_t b = b0; b < b1; ++b) mine += row_tiles(a, b, blockIdx.x == 0);
-        uint32_t incl = mine;
+    if constexpr (!LIST) {
+        const uint32_t unit = (gridDim.x - 1 - blockIdx.x) / splits, slot = unit / KVH;
+        uint32_t b = slot;
+        if (tid == 0) { at_h = unit % KVH; sm_bad[0] = sm_bad[1] = 0; }
+        if (a.tiled) {
+            if (tid == 0) at_b = a.c.B;
+            const uint32_t per = (a.c.B + blockDim.x - 1) / blockDim.x, b0 = min(a.c.B, tid * per), b1 = min(a.c.B, b0 + per);
+            uint32_t mine = 0;
+            for (uint32_t i = b0; i < b1; ++i) mine += row_tiles(a, i, blockIdx.x == 0);
+            uint32_t incl = mine;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) { const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= (uint32_t)o) incl += y; }
-        if (lane == 31) sums[warp] = incl;
-        __syncthreads();
-        uint32_t before = incl - mine;
-        for (uint32_t w = 0; w < warp; ++w) before += (uint32_t)sums[w];
-        if (slot >= before && slot < before + mine)
-            for (uint32_t b = b0; b < b1; ++b) {
-                const uint32_t n = row_tiles(a, b, false);
-                if (slot < before + n) { at_b = b; at_t = slot - before; break; }
-                before += n;
-            }
-        __syncthreads();
-        if (at_b == a.c.B) return;
-        r0 = at_t * kFewRows;
-        u0 = unit_of(a, at_b, r0);
+            for (int o = 1; o < 32; o <<= 1) { const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= (uint32_t)o) incl += y; }
+            if (lane == 31) sums[warp] = incl;
+            __syncthreads();
+            uint32_t before = incl - mine;
+            for (uint32_t w = 0; w < warp; ++w) before += (uint32_t)sums[w];
+            if (slot >= before && slot < before + mine)
+                for (uint32_t i = b0; i < b1; ++i) {
+                    const uint32_t n = row_tiles(a, i, false);
+                    if (slot < before + n) { at_b = i; at_t = slot - before; break; }
+                    before += n;
+                }
+            __syncthreads();
+            b = at_b;
+            if (b == a.c.B) return;                         // the whole cluster
+            r0 = at_t * kFewRows;
+        }
+        u0 = unit_of(a, b, r0);
+        if (u0.s.lost && at_h == 0 && tid == 0 && split == 0) note_bad_batch(a.status);
+        if (u0.tiles == 0) return;
         x0 = (unsigned long long)u0.tiles * split / splits; x1 = (unsigned long long)u0.tiles * (split + 1) / splits;
-        part += (size_t)split * a.c.T * a.H * dh; stat += (size_t)split * a.c.T * a.H;
         __syncthreads();
-        if (tid == 0) at_t = (uint32_t)x0;
+        if (tid == 0) { at_b = b; at_t = (uint32_t)x0; }
         __syncthreads();
     } else {
         const uint32_t per = (a.c.B + blockDim.x - 1) / blockDim.x, b0 = min(a.c.B, tid * per), b1 = min(a.c.B, b0 + per);
@@ -203,7 +212,7 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
     // ---- the copies: a cursor of their own, Stages - 1 tiles ahead ----
     uint32_t lb = at_b, lh = at_h, lt = at_t, left = (uint32_t)(x1 - x0), slot = 0;
     uint32_t no_page = 0;                                   // bit of a stage: a page was not there
-    Unit lu = TILED ? u0 : unit_of(a, lb, 0);
+    Unit lu = !LIST ? u0 : unit_of(a, lb, 0);
     auto request = [&]() {
         if (left) {
             const uint32_t j = lu.key(lt) + warp * kStep + (lane & 15u);
@@ -250,7 +259,7 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
     };
     // ---- the units of the stretch ----
     uint32_t b = at_b, h = at_h, t = at_t, todo = (uint32_t)(x1 - x0), use = 0, turn = 0;
-    Unit u = TILED ? u0 : unit_of(a, b, 0);
+    Unit u = !LIST ? u0 : unit_of(a, b, 0);
     for (;;) {
         const uint32_t t0 = t, t1 = min(u.tiles, t + todo), rows = min(u.s.n * a.rep - r0, ROWS);
         int pos[NR];
@@ -452,10 +461,10 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
         }
         if ((lost_page || u.bad) && lane == 0) sm_bad[turn] = 1;
         __syncthreads();
-        const bool bad = sm_bad[turn], all = TILED ? splits == 1 : t0 == 0 && t1 == u.tiles;
+        const bool bad = sm_bad[turn], all = LIST ? t0 == 0 && t1 == u.tiles : splits == 1;
         const size_t slot = 2 * (size_t)blockIdx.x + (t0 == 0);            // of a unit that began before: 0; that goes on behind: 1
-        float* const po = part + slot * ROWS * dh;
-        float2* const ps = stat + slot * ROWS;
+        float* const po = LIST ? part + slot * ROWS * dh : reinterpret_cast<float*>(smem);
+        float2* const ps = LIST ? stat + slot * ROWS : cta_ml;
         bool again = false;
         if (tid < dh) {
             for (uint32_t r = 0; r < rows; ++r) {
@@ -472,15 +481,12 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
                 if (bad) L = CUDART_NAN_F;
                 if (all) {
                     a.out[number_of(u, h, r0 + r) * dh + tid] = L == 0.f ? 0.f : x / L;
-                } else if (TILED) {
-                    part[number_of(u, h, r0 + r) * dh + tid] = x;
-                    if (tid == 0) stat[number_of(u, h, r0 + r)] = make_float2(M, L);
                 } else {
                     po[(size_t)r * dh + tid] = x;
                     if (tid == 0) ps[r] = make_float2(M, L);
                 }
             }
-            if (!TILED && bad)                              // more rows than were promised
+            if (!a.tiled && bad)                            // more rows than were promised
                 for (uint32_t r = rows; r < u.s.n * a.rep; ++r) a.out[number_of(u, h, r) * dh + tid] = CUDART_NAN_F;
         }
         if (bad && tid == 0) note_bad_batch(a.status);
@@ -488,9 +494,30 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
         if (__syncthreads_or(again && !bad)) {
             for (uint32_t r = warp; r < rows; r += kWarps) {
                 const size_t row = number_of(u, h, r0 + r);
-                float* to = all ? a.out + row * dh : TILED ? part + row * dh : po + (size_t)r * dh;
-                row_again<T>(a, b, h, u.s.first + (int)((r0 + r) / a.rep), u, t0, t1, a.q + row * dh, to, all ? nullptr : TILED ? stat + row : ps + r);
+                row_again<T>(a, b, h, u.s.first + (int)((r0 + r) / a.rep), u, t0, t1, a.q + row * dh, all ? a.out + row * dh : po + (size_t)r * dh, all ? nullptr : ps + r);
             }
+            if (!LIST) __syncthreads();
+        }
+        if constexpr (!LIST) {
+            if (splits == 1) return;
+            cluster_sync();
+            const uint32_t at_o = (uint32_t)__cvta_generic_to_shared(smem), at_ml = (uint32_t)__cvta_generic_to_shared(cta_ml);
+            for (uint32_t i = split * blockDim.x + tid; i < rows * dh; i += splits * blockDim.x) {
+                const uint32_t r = i / dh;
+                float M = -CUDART_INF_F, L = 0.f, y = 0.f;
+#pragma unroll 4
+                for (uint32_t k = 0; k < splits; k += 2) {  // a power of two, so two at a time
+                    const float2 m0 = ld_cta2(map_cta(at_ml + 8 * r, k)), m1 = ld_cta2(map_cta(at_ml + 8 * r, k + 1));
+                    const float x0 = ld_cta(map_cta(at_o + 4 * i, k)), x1 = ld_cta(map_cta(at_o + 4 * i, k + 1));
+                    const float mn = fmaxf(M, fmaxf(m0.x, m1.x)), base = mn == -CUDART_INF_F ? 0.f : mn, f = pow2(M - base), f0 = pow2(m0.x - base), f1 = pow2(m1.x - base);
+                    L = fmaf(L, f, fmaf(f0, m0.y, f1 * m1.y));
+                    y = fmaf(y, f, fmaf(f0, x0, f1 * x1));
+                    M = mn;
+                }
+                a.out[number_of(u, h, r0 + r) * dh + (i - r * dh)] = L == 0.f ? 0.f : y / L;
+            }
+            cluster_sync();                                 // nobody leaves while its shared memory is read
+            return;
         }
         turn ^= 1u;
         todo -= t1 - t0;
@@ -506,63 +533,113 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
 }
 
 // One CTA per stretch that begins inside a unit, of which the first of a unit merges all of its parts: the last of the CTA before, and the
-// first of its own and of those behind it. Rows over blockIdx.y; four threads per dim take every fourth part.
+// first of its own and of those behind it. Rows over blockIdx.y; four threads per dim take every fourth part, a thread per part its
+// weight. Bound by its trips to L2: the first 32 parts are on their way while the weights are worked out.
 constexpr uint32_t kMergeGroups = 4;
 __global__ void __launch_bounds__(kMergeGroups * 128) attn_few_merge_kernel(const __grid_constant__ AttnCall a, const float* part, const float2* stat, const Part* meta, uint32_t slot_rows) {
-    __shared__ float so[kMergeGroups][128];
-    __shared__ float2 sml[kMergeGroups];
+    constexpr uint32_t BATCH = 8, G = kMergeGroups, NT = G * 128;
+    static_assert(NT >= kFewCtas + 1, "a thread per part");
+    __shared__ float so[G][128], weight[NT];
+    __shared__ float2 sml[NT / 32];
     pdl_enter();
-    const uint32_t c = blockIdx.x + 1, r = blockIdx.y, d = threadIdx.x, grp = threadIdx.y, dh = a.c.dh;
+    const uint32_t c = blockIdx.x + 1, r = blockIdx.y, d = threadIdx.x, grp = threadIdx.y, tid = grp * 128 + d, dh = a.c.dh;
     const Part p = meta[c];
     if (p.b < 0 || !p.first) return;
     const KvSeq s = kv_seq(a.c, (uint32_t)p.b);
     if (r >= s.n * a.rep) return;
     const uint32_t parts = (uint32_t)p.last - c + 2;
-    float M = -CUDART_INF_F, L = 0.f, o = 0.f;
-    for (uint32_t i = grp; i < parts; i += kMergeGroups) {
-        const size_t row = (size_t)(2 * (c + i) - (i ? 2 : 1)) * slot_rows + r;        // i = 0: slot 1 of CTA c - 1; else slot 0 of CTA c + i - 1
-        const float2 ml = stat[row];
-        const float x = d < dh ? part[row * dh + d] : 0.f, mn = fmaxf(M, ml.x);
-        const float f = M == -CUDART_INF_F ? 0.f : pow2(M - mn), w = ml.x == -CUDART_INF_F ? 0.f : pow2(ml.x - mn);
-        o = fmaf(o, f, w * x); L = fmaf(L, f, w * ml.y);
-        M = mn;
+    auto row_of = [&](uint32_t i) { return (size_t)(2 * (c + i) - (i ? 2 : 1)) * slot_rows + r; };      // i = 0: slot 1 of CTA c - 1; else slot 0 of CTA c + i - 1
+    float v[BATCH];
+    auto request = [&](uint32_t i0) {
+#pragma unroll
+        for (uint32_t k = 0; k < BATCH; ++k)
+            if (i0 + G * k + grp < parts && d < dh) v[k] = __ldcg(part + row_of(i0 + G * k + grp) * dh + d);
+    };
+    request(0);
+    float2 ml = make_float2(-CUDART_INF_F, 0.f);
+    if (tid < parts) ml = __ldcg(stat + row_of(tid));
+    float M = ml.x;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    if (tid % 32 == 0) sml[tid / 32].x = M;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < NT / 32; ++i) M = fmaxf(M, sml[i].x);
+    const float w = ml.x == -CUDART_INF_F ? 0.f : pow2(ml.x - M);
+    weight[tid] = w;
+    float L = w * ml.y;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    if (tid % 32 == 0) sml[tid / 32].y = L;
+    __syncthreads();
+    float o = 0.f;
+    for (uint32_t i0 = 0; i0 < parts; i0 += G * BATCH) {
+        if (i0) request(i0);
+#pragma unroll
+        for (uint32_t k = 0; k < BATCH; ++k)
+            if (i0 + G * k + grp < parts) o = fmaf(weight[i0 + G * k + grp], v[k], o);
     }
     so[grp][d] = o;
-    if (d == 0) sml[grp] = make_float2(M, L);
     __syncthreads();
     if (grp || d >= dh) return;
-    M = -CUDART_INF_F; L = o = 0.f;
+    L = 0.f;
 #pragma unroll
-    for (uint32_t i = 0; i < kMergeGroups; ++i) M = fmaxf(M, sml[i].x);
+    for (uint32_t i = 0; i < NT / 32; ++i) L += sml[i].y;
+    o = 0.f;
 #pragma unroll
-    for (uint32_t i = 0; i < kMergeGroups; ++i) {
-        const float w = sml[i].x == -CUDART_INF_F ? 0.f : pow2(sml[i].x - M);
-        o = fmaf(w, so[i][d], o); L = fmaf(w, sml[i].y, L);
-    }
+    for (uint32_t i = 0; i < G; ++i) o += so[i][d];
     a.out[((size_t)(s.q0 + r / a.rep) * a.H + p.h * a.rep + r % a.rep) * dh + d] = L == 0.f ? 0.f : o / L;
 }
 
-template <typename T, int DHP, bool PAIR, bool TILED = false>
-bool ready_kernel() {
-    auto* kernel = attn_few_kernel<T, DHP, PAIR, TILED>;
-    static PerDevice<bool> ready;
+// How many clusters of 1, 2, 4, 8, 16 CTAs run at a time on the current device; nullptr (and the reason recorded) where that cannot be found out.
+struct Fits { int clusters[5]; };
+template <typename T, int DHP, bool PAIR>
+const Fits* prepare() {
+    using F = Few<T, DHP, PAIR>;
+    static PerDevice<Fits> device;
     int dev = -1;
-    if (cudaGetDevice(&dev) == cudaSuccess && ready.get(dev, [=](bool&) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Few<T, DHP, PAIR>::Smem) == cudaSuccess; }))
+    const Fits* fits = cudaGetDevice(&dev) != cudaSuccess ? nullptr : device.get(dev, [](Fits& f) {
+        auto* unit = attn_few_kernel<T, DHP, PAIR, false>;
+        auto* list = attn_few_kernel<T, DHP, PAIR, true>;
+        if (cudaFuncSetAttribute(unit, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)F::Smem) != cudaSuccess ||
+            cudaFuncSetAttribute(list, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)F::Smem) != cudaSuccess ||
+            cudaFuncSetAttribute(unit, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return false;
+        for (int i = 0; i < 5; ++i) {
+            cudaLaunchConfig_t c = {};
+            c.gridDim = dim3(1u << i); c.blockDim = dim3(32 * kWarps); c.dynamicSmemBytes = F::Smem;
+            cudaLaunchAttribute at;
+            at.id = cudaLaunchAttributeClusterDimension;
+            at.val.clusterDim.x = 1u << i; at.val.clusterDim.y = at.val.clusterDim.z = 1;
+            c.attrs = &at; c.numAttrs = 1;
+            if (cudaOccupancyMaxActiveClusters(&f.clusters[i], unit, &c) != cudaSuccess) { cudaGetLastError(); f.clusters[i] = 0; }
+        }
         return true;
-    return fail("attention: shared memory attribute: %s", cudaGetErrorString(cudaGetLastError()));
+    });
+    if (!fits) fail("attention: kernel attributes: %s", cudaGetErrorString(cudaGetLastError()));
+    return fits;
 }
 
 template <typename T, int DHP, bool PAIR>
 bool go(const AttnCall& a, float* scratch, cudaStream_t st) {
     using F = Few<T, DHP, PAIR>;
-    if (!ready_kernel<T, DHP, PAIR>()) return false;
+    const Fits* fits = prepare<T, DHP, PAIR>();
+    if (!fits) return false;
     const unsigned most = std::min(kFewCtas, (unsigned)device_sm_count() * F::PerSm);
-    const unsigned long long tiles = (unsigned long long)a.c.B * a.c.KVH * (((unsigned long long)(a.c.table ? a.c.cap : a.c.total) + kTile - 1) / kTile);
+    // the keys that a sequence can have in reach, as far as the host knows
+    const unsigned long long keys = a.c.table ? a.c.cap : a.c.total, seen = (unsigned long long)a.mask.window + a.mask.sinks + a.max_q;
+    const unsigned long long each = ((a.mask.window && seen < keys ? seen + 2 * kTile : keys) + kTile - 1) / kTile, units = (unsigned long long)a.c.B * a.c.KVH, tiles = units * each;
+    int cs = 4;
+    while (cs && ((units << cs) > most || fits->clusters[cs] < (int)units || (1ull << cs) >= 2 * each)) --cs;
+    if ((units << cs) <= most && (each + (1u << cs) - 1) / (1u << cs) <= (tiles + most - 1) / most + kClusterTiles) {
+        if (!launch_units(attn_few_kernel<T, DHP, PAIR, false>, (unsigned)units, 1u << cs, 32 * kWarps, F::Smem, st, a, (float*)nullptr, (float2*)nullptr, (Part*)nullptr, 1u << cs)) return false;
+        note_launch();
+        return check_launch("attn_few");
+    }
     const unsigned grid = tiles < most ? (unsigned)std::max(tiles, 1ull) : most;
     Part* meta = reinterpret_cast<Part*>(scratch);
     float2* stat = reinterpret_cast<float2*>(meta + kFewCtas);
     float* part = reinterpret_cast<float*>(stat + 2 * kFewCtas * F::Rows);
-    launch_overlapped(attn_few_kernel<T, DHP, PAIR, false>, dim3(grid), dim3(32 * kWarps), F::Smem, st, a, part, stat, meta, 1u);
+    launch_overlapped(attn_few_kernel<T, DHP, PAIR, true>, dim3(grid), dim3(32 * kWarps), F::Smem, st, a, part, stat, meta, 1u);
     note_launch();
     if (!check_launch("attn_few")) return false;
     if (grid == 1) return true;
@@ -573,23 +650,22 @@ bool go(const AttnCall& a, float* scratch, cudaStream_t st) {
 }
 
 template <int DHP>
-bool go_tiled(const AttnCall& a, const ChunkPlan& pl, float* scratch, cudaStream_t st) {
-    using F = Few<float, DHP, false>;
-    if (!ready_kernel<float, DHP, false, true>()) return false;
-    const unsigned long long ctas = (unsigned long long)a.c.KVH * pl.splits * pl.slots;
-    if (ctas > 0x7fffffffull) return fail("attention: %llu tiles of query rows", ctas);
-    float* part = scratch;
-    float2* stat = reinterpret_cast<float2*>(part + (size_t)pl.splits * a.c.T * a.H * a.c.dh);
-    launch_overlapped(attn_few_kernel<float, DHP, false, true>, dim3((unsigned)ctas), dim3(32 * kWarps), F::Smem, st, a, part, stat, (Part*)nullptr, pl.splits);
+bool go_tiled(const AttnCall& a, const ChunkPlan& pl, cudaStream_t st) {
+    const Fits* fits = prepare<float, DHP, false>();
+    if (!fits) return false;
+    const unsigned long long units = (unsigned long long)a.c.KVH * pl.slots;
+    if (units * pl.splits > 0x7fffffffull) return fail("attention: %llu tiles of query rows", units);
+    if (!launch_units(attn_few_kernel<float, DHP, false, false>, (unsigned)units, pl.splits, 32 * kWarps, Few<float, DHP, false>::Smem, st, a, (float*)nullptr, (float2*)nullptr,
+                      (Part*)nullptr, pl.splits)) return false;
     note_launch();
-    return check_launch("attn_tiled") && (pl.splits == 1 || launch_attn_merge(a, pl.splits, part, stat, st));
+    return check_launch("attn_tiled");
 }
 
 }  // namespace
 
-bool launch_attn_tiled(AttnCall a, const ChunkPlan& pl, float* scratch, cudaStream_t st) {
+bool launch_attn_tiled(AttnCall a, const ChunkPlan& pl, cudaStream_t st) {
     a.tiled = true;
-    return a.c.dh <= 64 ? go_tiled<64>(a, pl, scratch, st) : go_tiled<128>(a, pl, scratch, st);
+    return a.c.dh <= 64 ? go_tiled<64>(a, pl, st) : go_tiled<128>(a, pl, st);
 }
 
 size_t attn_few_scratch(uint32_t rows, uint32_t dh) {

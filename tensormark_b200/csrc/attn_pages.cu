@@ -5,7 +5,6 @@
 #include "common.cuh"
 #include "state.h"
 
-#include <algorithm>
 #include <cmath>
 
 namespace tmc {
@@ -42,16 +41,13 @@ Split split(unsigned B, unsigned long long rows, unsigned rep) {
     return Split{B == 1 || rep > kFewRows ? 0u : rep <= 8 ? 8u : kFewRows, true};
 }
 
-size_t few_bytes(Split sp, unsigned dh) { return sp.few ? attn_few_scratch(sp.few, dh) : 0; }
-
 bool launch(AttnCall a, bool half, float* scratch, cudaStream_t st) {
     const Split sp = split(a.c.B, (unsigned long long)a.max_q * a.rep, a.rep);
     a.few = sp.few; a.others = sp.others; a.status = device_status_word();
     if (sp.few && !launch_attn_few(a, half, scratch, st)) return false;
     if (!sp.others) return true;
     const ChunkPlan pl = plan_attn_chunk(a.c.T, a.c.B, a.c.KVH, a.rep, a.few, half ? kChunkRows : kFewRows);
-    float* own = scratch + few_bytes(sp, a.c.dh) / sizeof(float);
-    return half ? launch_attn_chunk(a, pl, own, st) : launch_attn_tiled(a, pl, own, st);
+    return half ? launch_attn_chunk(a, pl, st) : launch_attn_tiled(a, pl, st);
 }
 
 }  // namespace
@@ -65,10 +61,7 @@ size_t tm_cuda_attn_paged_scratch(unsigned T, unsigned B, unsigned max_q, unsign
     if (!KVH || !H || H % KVH || !dh || !T) return 16;
     const unsigned rep = H / KVH;
     const Split sp = split(B, (unsigned long long)(max_q && max_q < T ? max_q : T) * rep, rep);
-    size_t chunk = 0;
-    if (sp.others)                                              // of either type of cache
-        for (const uint32_t tile : {kChunkRows, kFewRows}) chunk = std::max(chunk, attn_chunk_scratch(plan_attn_chunk(T, B, KVH, rep, sp.few, tile), T, H, dh));
-    return std::max<size_t>(16, few_bytes(sp, dh) + chunk);
+    return sp.few ? attn_few_scratch(sp.few, dh) : 16;
 }
 size_t tm_cuda_attn_window_scratch(unsigned T, unsigned H, unsigned KVH, unsigned dh) { return tm_cuda_attn_paged_scratch(T, 1, T, H, KVH, dh); }
 

@@ -25,11 +25,10 @@ size_t attn_few_scratch(uint32_t rows, uint32_t dh);
 bool launch_attn_few(const AttnCall& a, bool half, float* scratch, cudaStream_t st);
 
 // Sequences with more rows, in tiles of row_tile: 256 over fp16 caches (attn_chunk.cu), 16 over fp32 ones (attn_few.cu).
-struct ChunkPlan { uint32_t slots, splits; };           // (sequence, tile of rows) at most; parts that the keys of one are split into
+// The keys of a tile of rows are split over the CTAs of a cluster, which merge: as many as keep the SMs busy, a power of two up to 8.
+struct ChunkPlan { uint32_t slots, splits; };           // (sequence, tile of rows) at most; parts
 ChunkPlan plan_attn_chunk(uint32_t T, uint32_t B, uint32_t KVH, uint32_t rep, uint32_t few, uint32_t row_tile);
-size_t attn_chunk_scratch(const ChunkPlan& pl, uint32_t T, uint32_t H, uint32_t dh);
-bool launch_attn_chunk(const AttnCall& a, const ChunkPlan& pl, float* scratch, cudaStream_t st);
-bool launch_attn_tiled(AttnCall a, const ChunkPlan& pl, float* scratch, cudaStream_t st);
-bool launch_attn_merge(const AttnCall& a, uint32_t splits, const float* part, const float2* stat, cudaStream_t st);
+bool launch_attn_chunk(const AttnCall& a, const ChunkPlan& pl, cudaStream_t st);
+bool launch_attn_tiled(AttnCall a, const ChunkPlan& pl, cudaStream_t st);
 
 }  // namespace tmc

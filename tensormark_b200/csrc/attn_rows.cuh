@@ -17,6 +17,32 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t b
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
+// The parts of a row that the CTAs of a cluster hold lie at the same place in the shared memory of each.
+__device__ __forceinline__ uint32_t map_cta(uint32_t at, uint32_t rank) {
+    uint32_t v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(v) : "r"(at), "r"(rank));
+    return v;
+}
+__device__ __forceinline__ float2 ld_cta2(uint32_t at) {
+    float2 f;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(f.x), "=f"(f.y) : "r"(at) : "memory");
+    return f;
+}
+__device__ __forceinline__ float ld_cta(uint32_t at) {
+    float f;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(at) : "memory");
+    return f;
+}
+__device__ __forceinline__ float4 ld_cta4(uint32_t at) {
+    float4 f;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(at) : "memory");
+    return f;
+}
+__device__ __forceinline__ void cluster_sync() {            // by whole warps
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 // The keys [0, a) and [b, end) in tiles of N that start at multiples of N: tile t at key t * N, from `head` on at (t + skip) * N.
 // At least one, so that rows that see nothing are visited.
 template <uint32_t N> struct KeyTiles {
@@ -32,7 +58,7 @@ template <uint32_t N> struct KeyTiles {
 };
 
 // One row over tiles [t0, t1) by one warp, key by key in fp32: what a kernel whose products take masked values along computes again
-// where a value was not finite. stat: the row stays unnormalised, with its maximum and sum there.
+// where a value was not finite. stat: the row stays unnormalised, with its maximum and sum there; nullptr: it is finished.
 template <typename T, uint32_t N>
 __device__ __noinline__ void row_again(const AttnCall& a, uint32_t b, uint32_t h, int p, KeyTiles<N> tiles, uint32_t t0, uint32_t t1, const float* q, float* to, float2* stat) {
     const uint32_t lane = threadIdx.x & 31u, dh = a.c.dh;
