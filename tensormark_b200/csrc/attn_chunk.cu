@@ -127,7 +127,6 @@ __device__ __forceinline__ void parts(float x, float y, uint32_t& hi, uint32_t& 
         "fma.rn.f32.f16 %0, l, m, %3;\n\tfma.rn.f32.f16 %1, h, m, %4;\n\t}" : "=f"(u), "=f"(v) : "r"(hi), "f"(x), "f"(y));
     lo = half2_bits(u, v);
 }
-__device__ __forceinline__ int window_from(const KvMask& m, int p) { return m.window && p >= (int)m.window ? p - (int)m.window + 1 : 0; }
 // Is key j hidden from position p, whose window begins at lo?
 __device__ __forceinline__ bool hidden(int j, int p, int lo, int sinks) { return (j > p) | ((j < lo) & (j >= sinks)); }
 
@@ -289,9 +288,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
             auto look_up = [&](uint32_t j) {
 #pragma unroll
                 for (uint32_t r = 0; r < 4; ++r) {
-                    const uint32_t key = kt.key(t0 + j) + 32 * r + lane;
+                    const uint32_t place_at = (t0 + j) * kKeys + 32 * r + lane;
                     page[r] = 0;
-                    if (a.c.table && j < n && key < kt.end) page[r] = (uint32_t)a.c.table[(size_t)b * a.c.table_ld + slot_of(key)];
+                    if (a.c.table && j < n && place_at < kt.count) page[r] = (uint32_t)a.c.table[(size_t)b * a.c.table_ld + slot_of(kt.key(place_at))];
                 }
             };
             look_up(0);
@@ -299,8 +298,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
                 uint32_t lo[4], hi[4], there[4];
 #pragma unroll
                 for (uint32_t r = 0; r < 4; ++r) {
-                    const uint32_t key = kt.key(t0 + j) + 32 * r + lane;
-                    bool have = key < kt.end;
+                    const uint32_t place_at = (t0 + j) * kKeys + 32 * r + lane, key = kt.key(place_at);
+                    bool have = place_at < kt.count;
                     if (have && page[r] >= a.c.npages) { have = false; missing = true; }
                     const uint32_t row = a.c.table ? key - slot_of(key) * a.c.page : key;
                     const size_t at = have ? (((size_t)page[r] * a.c.KVH + h) * a.c.page + row) * dh * 2 : 0;
@@ -392,18 +391,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             }
             // S of the tiles that not every row of the warp sees whole: what a row does not see is -infinity from here on
-            auto hide = [&](int j0) {
+            auto hide = [&](uint32_t u0) {
                 const int p = place[row], lo = window_from(a.mask, p), sinks = (int)a.mask.sinks;
 #pragma unroll 1
                 for (uint32_t c = 0; c < kKeys / 16; ++c) {
-                    const int i0 = j0 + (int)(16 * c);
-                    if (i0 + 15 <= p_min && (i0 >= lo_max || i0 + 16 <= sinks)) continue;
+                    const uint32_t u1 = u0 + 16 * c;
+                    if (kt.seen(u1, 16, p_min, (uint32_t)lo_max)) continue;
                     uint32_t v[16];
                     tmem_ld(st + 16 * c, v);
                     tmem_landed(v);
 #pragma unroll
                     for (uint32_t k = 0; k < 16; ++k)
-                        v[k] = hidden(i0 + (int)k, p, lo, sinks) ? 0xff800000u : v[k];
+                        v[k] = hidden((int)kt.key(u1 + k), p, lo, sinks) ? 0xff800000u : v[k];
                     tmem_st(st + 16 * c, v);
                 }
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -461,9 +460,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
             for (uint32_t j = 0; j < n; ++j) {
                 if (!wait_for(bars.done[w], j & 1u, &gone)) { ok = false; break; }
                 fence_after();
-                const int j0 = (int)kt.key(t0 + j);
-                const bool whole = j0 + (int)kKeys - 1 <= p_min && (j0 >= lo_max || j0 + (int)kKeys <= (int)a.mask.sinks);
-                if (!whole) hide(j0);
+                if (!kt.seen((t0 + j) * kKeys, kKeys, p_min, (uint32_t)lo_max)) hide((t0 + j) * kKeys);
                 const float mn = fmaxf(m, maximum() * back), base = mn == -CUDART_INF_F ? 0.f : mn, now = pow2(m - base);
                 m = mn;
                 weights(base, now);

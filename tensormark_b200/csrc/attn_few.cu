@@ -90,7 +90,8 @@ struct Part { int b, h, last, first; };     // of CTA c: the unit in whose middl
 template <typename T, int DHP, bool PAIR> struct Few {
     static constexpr uint32_t Rows = PAIR ? 8 : 16;
     static constexpr uint32_t RowBytes = DHP * sizeof(T), StageBytes = 2 * kStep * RowBytes;     // K and V of a warp's step
-    static constexpr uint32_t Stages = sizeof(T) == 4 ? (DHP == 128 ? (PAIR ? 3 : 2) : 4) : (PAIR ? 3 : 2) * (128 / DHP);
+    // two CTAs per SM where their rings fit: 700 tokens of 32 / 4 heads of 64 in fp32 take 144 us with one (four stages), 84 with two (three)
+    static constexpr uint32_t Stages = sizeof(T) == 4 ? (DHP == 128 && !PAIR ? 2 : 3) : (PAIR ? 3 : 2) * (128 / DHP);
     static constexpr uint32_t Ring = kWarps * Stages * StageBytes, Merge = kWarps * Rows * DHP * 4;
     static constexpr uint32_t Smem = Ring + Merge;
     static constexpr uint32_t PerSm = Smem <= 114688 ? 2 : 1;
@@ -215,11 +216,11 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
     Unit lu = !LIST ? u0 : unit_of(a, lb, 0);
     auto request = [&]() {
         if (left) {
-            const uint32_t j = lu.key(lt) + warp * kStep + (lane & 15u);
+            const uint32_t place = lt * kTile + warp * kStep + (lane & 15u);
             size_t at = 0;
-            const bool in = j < lu.end;
+            const bool in = place < lu.count;
             bool ok = true;
-            if (in) ok = kv_row(a.c, lb, j, &at);
+            if (in) ok = kv_row(a.c, lb, lu.key(place), &at);
             no_page = no_page & ~(1u << slot) | (__any_sync(0xffffffffu, !ok) ? 1u << slot : 0u);
             at = (at + (size_t)lh * a.c.page * dh) * sizeof(T);
             const uint32_t chunks = dh * (uint32_t)sizeof(T) / 16, lo = (uint32_t)at, hi = (uint32_t)(at >> 32);
@@ -310,14 +311,15 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
             for (uint32_t k = 0; k < 2 * NR; ++k) o[i][k] = 0.f;
         bool lost_page = false;
         const int p_least = u.s.first + (int)(r0 / a.rep);
+        const uint32_t from = (uint32_t)window_from(a.mask, (int)u.end - 1);       // the last row's window begins last
 
         for (; t < t1; ++t) {
             request();
             asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
             __syncwarp();
-            const uint32_t kat = ring + use * SB, vat = kat + kStep * RB, j0 = u.key(t) + warp * kStep;
+            const uint32_t kat = ring + use * SB, vat = kat + kStep * RB, u0 = t * kTile + warp * kStep;        // the first place of this warp's step
             if (no_page >> use & 1u) lost_page = true;
-            if (j0 < u.end) {
+            if (u0 < u.count) {
                 float s[2][4] = {};
                 if constexpr (kHalf) {
                     const uint32_t key = (lane >> 4) * 8 + (lane & 7u), row = kat + key * RB, c0 = lane >> 3 & 1u;
@@ -353,8 +355,7 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
                         }
                     }
                 }
-                const bool whole = (int)j0 + (int)kStep - 1 <= p_least &&
-                                   (!a.mask.window || j0 + a.mask.window >= u.end || j0 + kStep <= a.mask.sinks);
+                const bool whole = u.seen(u0, kStep, p_least, from);
                 float corr[NR];
                 uint32_t ph[NR][4];                         // the weights as the second product's rows: PAIR: [0] both parts; else high, low
 #pragma unroll
@@ -368,7 +369,7 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
                     if (!whole) {
 #pragma unroll
                         for (uint32_t i = 0; i < 4; ++i)
-                            if (!kv_sees(a.mask, pos[n], (int)(j0 + (i >> 1) * 8 + 2 * t4 + (i & 1)))) x[i] = -CUDART_INF_F;
+                            if (!kv_sees(a.mask, pos[n], (int)u.key(u0 + (i >> 1) * 8 + 2 * t4 + (i & 1)))) x[i] = -CUDART_INF_F;
                     }
                     float mn = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
                     mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 1));

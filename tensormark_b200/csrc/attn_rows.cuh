@@ -17,6 +17,9 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t b
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
+// Where the window of a row at p begins
+__device__ __forceinline__ int window_from(const KvMask& m, int p) { return m.window && p >= (int)m.window ? p - (int)m.window + 1 : 0; }
+
 // The parts of a row that the CTAs of a cluster hold lie at the same place in the shared memory of each.
 __device__ __forceinline__ uint32_t map_cta(uint32_t at, uint32_t rank) {
     uint32_t v;
@@ -43,18 +46,21 @@ __device__ __forceinline__ void cluster_sync() {            // by whole warps
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// The keys [0, a) and [b, end) in tiles of N that start at multiples of N: tile t at key t * N, from `head` on at (t + skip) * N.
-// At least one, so that rows that see nothing are visited.
+// The keys [0, a) and [b, e) that a set of rows sees, one behind the other, in tiles of N places: a window's keys follow the first ones in
+// the same tile. At least one tile, so that rows that see nothing are visited.
 template <uint32_t N> struct KeyTiles {
-    uint32_t tiles, head, skip, end;
+    uint32_t tiles, count, a, skip;                         // places; the first that lies `skip` keys further on
+    uint32_t end;                                           // no row is at a position from here on
     __device__ __forceinline__ void set(const KvSpan& sp, bool none) {
-        end = none ? 0u : sp.e;
-        const uint32_t e = (end + N - 1) / N, lo = sp.b / N;
-        head = (sp.a + N - 1) / N;
-        skip = lo > head ? lo - head : 0u;
-        tiles = max(1u, e - min(e, skip));
+        a = sp.a; skip = sp.b - sp.a; end = none ? 0u : sp.e;
+        count = none ? 0u : sp.e - min(sp.e, skip);
+        tiles = max(1u, (count + N - 1) / N);
     }
-    __device__ __forceinline__ uint32_t key(uint32_t t) const { return (t < head ? t : t + skip) * N; }
+    __device__ __forceinline__ uint32_t key(uint32_t place) const { return place + (place < a ? 0u : skip); }
+    // Does a row at p_least or behind it, in a window that begins at `from` or before it, see all of the places [u, u + n)?
+    __device__ __forceinline__ bool seen(uint32_t u, uint32_t n, int p_least, uint32_t from) const {
+        return (int)key(u + n - 1) <= p_least && (u + n <= a || key(max(u, a)) >= from);
+    }
 };
 
 // One row over tiles [t0, t1) by one warp, key by key in fp32: what a kernel whose products take masked values along computes again
@@ -68,8 +74,8 @@ __device__ __noinline__ void row_again(const AttnCall& a, uint32_t b, uint32_t h
 #pragma unroll
     for (int k = 0; k < 4; ++k) qr[k] = lane + 32u * k < dh ? q[lane + 32u * k] * (a.scale * kLog2e) : 0.f;
     for (uint32_t t = t0; t < t1; ++t) {
-        const uint32_t j0 = tiles.key(t);
-        for (uint32_t j = j0; j < min(j0 + N, tiles.end); ++j) {
+        for (uint32_t u = t * N; u < min((t + 1) * N, tiles.count); ++u) {
+            const uint32_t j = tiles.key(u);
             size_t at;
             if (!kv_sees(a.mask, p, (int)j) || !kv_row(a.c, b, j, &at)) continue;
             float x = 0.f;

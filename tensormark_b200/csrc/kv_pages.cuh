@@ -99,7 +99,7 @@ __device__ __forceinline__ void kv_note_lost(const KvBatch& c, int* status) {
 struct KvMask { uint32_t window, sinks; };
 inline KvMask kv_mask(unsigned window, unsigned sinks) { return KvMask{window > 0x7fffffffu ? 0u : window, sinks > 0x7fffffffu ? 0x7fffffffu : sinks}; }
 TM_HD bool kv_sees(const KvMask& m, int p, int j) {
-    return j <= p && (!m.window || (int)m.window > p - j || j < (int)m.sinks);
+    return (j <= p) & (!m.window | ((int)m.window > p - j) | (j < (int)m.sinks));     // without branches
 }
 // The keys that positions [p0, p1] see between them: [0, a) and [b, e), a <= b.
 struct KvSpan { uint32_t a, b, e; };
