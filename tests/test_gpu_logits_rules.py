@@ -94,6 +94,19 @@ def test_rules(cuda, torch_mod, B, V, n, k, masked):
     run(cuda, torch_mod, x, V, a, in_place=True, shift=3)
 
 
+@pytest.mark.parametrize("V", list(range(1018, 1030)) + [4094, 4095, 8190, 8191])
+def test_slices_that_end_anywhere(cuda, torch_mod, V):
+    """Every alignment of rows against slices: last slices of one logit, and ones that the row does not reach."""
+    rng = np.random.default_rng(V)
+    for B in (1, 200 if V < 2000 else 160):
+        for shift in (0, 1, 2, 3):
+            x, a = case(rng, B, V, 40, 6, True, V + shift)
+            a["tokens"][:, :4] = V - 1 - np.arange(4)
+            a["bias_ids"][:, 0] = V - 1
+            a["n_tokens"][:], a["n_bias"][:] = 40, 6
+            run(cuda, torch_mod, x, V, a, in_place=True, shift=shift)
+
+
 def test_each_rule_alone(cuda, torch_mod):
     rng = np.random.default_rng(0)
     x, a = case(rng, 3, 5000, 64, 9, True, 5000)
