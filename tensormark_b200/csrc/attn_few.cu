@@ -265,7 +265,9 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
         const uint32_t t0 = t, t1 = min(u.tiles, t + todo), rows = min(u.s.n * a.rep - r0, ROWS);
         int pos[NR];
         float back[NR], m[NR], l[NR], o[NB][2 * NR];        // back: what undoes q's power of two
-        uint32_t qf[NR][KS][4];                             // fp16: the fragments, both parts; fp32: the values of a row
+        uint32_t qf[NR][KS][4];                             // fp16: the fragments, both parts; fp32: the values of a row, or their high parts
+        constexpr bool KEEP = !kHalf && DHP == 64;          // fp32: q's low parts are kept too, where registers are left
+        uint32_t qlow[KEEP ? NR : 1][KEEP ? KS : 1][4];
         {
             const float* qp[NR];
 #pragma unroll
@@ -301,7 +303,12 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
                     }
                 } else {
 #pragma unroll
-                    for (uint32_t k = 0; k < 2 * KS; ++k) { qf[n][k / 2][2 * (k & 1)] = __float_as_uint(raw[k].x); qf[n][k / 2][2 * (k & 1) + 1] = __float_as_uint(raw[k].y); }
+                    for (uint32_t k = 0; k < 2 * KS; ++k) {
+                        if constexpr (KEEP) {
+                            parts(raw[k].x, qf[n][k / 2][2 * (k & 1)], qlow[n][k / 2][2 * (k & 1)]);
+                            parts(raw[k].y, qf[n][k / 2][2 * (k & 1) + 1], qlow[n][k / 2][2 * (k & 1) + 1]);
+                        } else { qf[n][k / 2][2 * (k & 1)] = __float_as_uint(raw[k].x); qf[n][k / 2][2 * (k & 1) + 1] = __float_as_uint(raw[k].y); }
+                    }
                 }
             }
         }
@@ -336,9 +343,9 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
                         uint32_t ah[4], al[4];              // PAIR: ah holds both parts
 #pragma unroll
                         for (uint32_t n = 0; n < NR; ++n) {
-                            uint32_t h0, l0, h1, l1;
-                            parts(__uint_as_float(qf[n][k / 2][2 * (k & 1)]), h0, l0);
-                            parts(__uint_as_float(qf[n][k / 2][2 * (k & 1) + 1]), h1, l1);
+                            uint32_t h0 = qf[n][k / 2][2 * (k & 1)], h1 = qf[n][k / 2][2 * (k & 1) + 1], l0, l1;
+                            if constexpr (KEEP) { l0 = qlow[n][k / 2][2 * (k & 1)]; l1 = qlow[n][k / 2][2 * (k & 1) + 1]; }
+                            else { parts(__uint_as_float(h0), h0, l0); parts(__uint_as_float(h1), h1, l1); }
                             if constexpr (PAIR) { ah[0] = h0; ah[1] = l0; ah[2] = h1; ah[3] = l1; }
                             else { ah[n] = h0; al[n] = l0; ah[2 + n] = h1; al[2 + n] = l1; }
                         }
