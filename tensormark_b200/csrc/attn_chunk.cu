@@ -35,6 +35,9 @@ template <int DHP> struct Chunk {
     static constexpr uint32_t Tile = kKeys * DHP * 2;      // bytes of a tile of keys, or of one part of q; 64 dims are 128 bytes
     static constexpr uint32_t Half = kKeys * 128;
     static constexpr uint32_t Buffers = DHP == 128 ? 3 : 6;
+    // registers of the warps that issue and of those that hold rows: of the 384 x 168 that the block is launched with
+    static constexpr uint32_t RegsIssue = DHP == 128 ? 56 : 104, RegsRows = DHP == 128 ? 224 : 200;
+    static_assert(RegsIssue + 2 * RegsRows <= 3 * 168);
     static constexpr uint32_t Smem = 4 * Tile + Buffers * Tile + 1024;        // q: two tiles of two parts
 };
 
@@ -228,7 +231,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
     bool ok = true;
 
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::RegsIssue));
         if (warp == kWarpMma && n) {
             const uint32_t lead = elect_one();
             constexpr uint32_t idesc_s = (1u << 4) | ((kKeys >> 3) << 17) | ((kRows >> 4) << 24);                    // fp16 x fp16 -> fp32
@@ -327,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
             if (missing) bad_page = 1;
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::RegsRows));
         const uint32_t w = (warp - 4) >> 2, r = (warp & 3u) * 32 + lane, row = w * kRows + r;
         if (w < tiles2) {
             int p_min, lo_max;                                           // the least that a row of the warp sees ahead and behind
