@@ -55,9 +55,9 @@ __device__ __forceinline__ void parts(float x, float y, uint32_t& hi, uint32_t& 
     hi = *reinterpret_cast<const uint32_t*>(&h);
     lo = half2_bits(x - f.x, y - f.y);
 }
-__device__ __forceinline__ void parts(float x, uint32_t& hi, uint32_t& lo) {             // tf32: the low part is cut to 11 bits by the product
+__device__ __forceinline__ void parts(float x, uint32_t& hi, uint32_t& lo) {             // as tf32, both rounded: the product would cut
     asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
-    lo = __float_as_uint(x - __uint_as_float(hi));
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
 }
 
 // ---- the list of work ------------------------------------------------------------------------------------------------
@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
             const uint32_t kat = ring + use * SB, vat = kat + kStep * RB, u0 = t * kTile + warp * kStep;        // the first place of this warp's step
             if (no_page >> use & 1u) lost_page = true;
             if (u0 < u.count) {
-                float s[2][4] = {};
+                float s[2][4] = {}, low[2][4] = {};         // what the low parts add is summed apart: every step cuts the sum that it adds to
                 if constexpr (kHalf) {
                     const uint32_t key = (lane >> 4) * 8 + (lane & 7u), row = kat + key * RB, c0 = lane >> 3 & 1u;
 #pragma unroll
@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
                         uint32_t f[4];
                         ldsm4(f, row + (((2 * k + c0) ^ (key & 7u)) << 4));
 #pragma unroll
-                        for (uint32_t n = 0; n < NR; ++n) { mma_f16(s[0], qf[n][k], f[0], f[1]); mma_f16(s[1], qf[n][k], f[2], f[3]); }
+                        for (uint32_t n = 0; n < NR; ++n) { mma_f16(n ? low[0] : s[0], qf[n][k], f[0], f[1]); mma_f16(n ? low[1] : s[1], qf[n][k], f[2], f[3]); }
                     }
                 } else {
 #pragma unroll
@@ -357,10 +357,14 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
                             uint32_t h0, l0, h1, l1;
                             parts(f.x, h0, l0); parts(f.y, h1, l1);
                             mma_tf32(s[nb], ah, h0, h1);
-                            mma_tf32(s[nb], ah, l0, l1);
-                            if constexpr (!PAIR) mma_tf32(s[nb], al, h0, h1);
+                            mma_tf32(low[nb], ah, l0, l1);
+                            if constexpr (!PAIR) mma_tf32(low[nb], al, h0, h1);
                         }
                     }
+                }
+                if constexpr (!kHalf || !PAIR) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; ++i) s[i >> 2][i & 3] += low[i >> 2][i & 3];
                 }
                 const bool whole = u.seen(u0, kStep, p_least, from);
                 float corr[NR];
