@@ -169,10 +169,10 @@ bool tm_cuda_attn_decode_static_dev(const float* q, const void* kc, const void* 
  * p % page of page table[b * table_ld + p / page]; entries that no position needs may hold anything. All arrays are device memory
  * of the library's device, read when the kernels run: a captured graph may be replayed with other contents. The calls refuse what
  * the host can see. What only the device sees is checked there: a page, length or range of rows that is out of range is
- * not read or written, the rows of out that depend on it are NaN (rows that belong to no sequence: left as they are), and
- * the next synchronising entry of the lane reports it. A new token before position 0 (more new tokens than kv_len says) is not stored,
+ * not read or written, the rows of out that depend on it are NaN, other rows of the same sequence may be (rows that belong to no
+ * sequence: left as they are), and the next synchronising entry of the lane after the kernels reports it. A new token before position 0 (more new tokens than kv_len says) is not stored,
  * and sees no key.
- * No call allocates or synchronises. Calls may run at the same time on several streams if each has its own scratch; a graph
+ * No call allocates or synchronises (the library's own first call aside: tm_cuda_init). Calls may run at the same time on several streams if each has its own scratch; a graph
  * keeps using the scratch that it was captured with. */
 typedef struct tm_cuda_kv_pages {
     void* k;                     /* [npages][KVH][page][dh], half when kv_half != 0, else fp32; on 16-byte boundaries */
@@ -192,7 +192,8 @@ bool tm_cuda_kv_append_paged_dev(const tm_cuda_kv_pages* kv, const float* qkv, f
                                  unsigned rope_rows, void* stream);
 /* out[t] = softmax(scale q k) v over the keys j that the position p of token t sees: j <= p, and with window > 0 also
  * j > p - window or j < sinks. A token that sees none: zeros. q, out: [T][H * dh] fp32; sums and statistics in fp32, results as from
- * fp32 products with both cache types. max_q: the most new tokens that one sequence has (0: not known, T); a sequence with more is
+ * fp32 products with both cache types. Values and keys that a token does not see do not count, whatever they are; where a result
+ * is not finite the row is computed again key by key, which is slow. out must not overlap q. max_q: the most new tokens that one sequence has (0: not known, T); a sequence with more is
  * treated as out of range. `scratch` holds tm_cuda_attn_paged_scratch(...) bytes; what it holds before does not matter. */
 size_t tm_cuda_attn_paged_scratch(unsigned T, unsigned B, unsigned max_q, unsigned H, unsigned KVH, unsigned dh);
 bool tm_cuda_attn_paged_dev(const tm_cuda_kv_pages* kv, const float* q, float* scratch, size_t scratch_bytes, float* out, unsigned T,

@@ -642,7 +642,9 @@ bool go(const AttnCall& a, float* scratch, cudaStream_t st) {
     const unsigned long long each = ((a.mask.window && seen < keys ? seen + 2 * kTile : keys) + kTile - 1) / kTile, units = (unsigned long long)a.c.B * a.c.KVH, tiles = units * each;
     int cs = 4;
     while (cs && ((units << cs) > most || fits->clusters[cs] < (int)units || (1ull << cs) >= 2 * each)) --cs;
-    if ((units << cs) <= most && (each + (1u << cs) - 1) / (1u << cs) <= (tiles + most - 1) / most + kClusterTiles) {
+    // of several sequences some may be short, which evens out over a list and not over clusters
+    const unsigned long long listed = a.c.B == 1 ? (tiles + most - 1) / most : 1;
+    if ((units << cs) <= most && (each + (1u << cs) - 1) / (1u << cs) <= listed + kClusterTiles) {
         if (!launch_units(attn_few_kernel<T, DHP, PAIR, false>, (unsigned)units, 1u << cs, 32 * kWarps, F::Smem, st, a, (float*)nullptr, (float2*)nullptr, (Part*)nullptr, 1u << cs)) return false;
         note_launch();
         return check_launch("attn_few");

@@ -74,6 +74,7 @@ bool tm_cuda_attn_paged_dev(const tm_cuda_kv_pages* kv, const float* q, float* s
     if (!(scale > 0.f) || !std::isfinite(scale)) return fail("attn_paged: the scale is not a positive number");
     const size_t need = tm_cuda_attn_paged_scratch(T, c.B, max_q, H, c.KVH, c.dh);
     if (scratch_bytes < need) return fail("attn_paged: %zu bytes of scratch, %zu are needed", scratch_bytes, need);
+    if (overlap(q, (size_t)T * H * c.dh * 4, out, (size_t)T * H * c.dh * 4)) return fail("attn_paged: out overlaps q");
     if (!on_library_device("attn_paged")) return false;
     if (!T) return true;
     return launch(AttnCall{c, kv_mask(window, sinks), q, out, H, H / c.KVH, max_q && max_q < T ? max_q : T, 0, false, scale, nullptr, false}, kv->kv_half != 0, scratch, (cudaStream_t)stream);
@@ -91,6 +92,7 @@ bool tm_cuda_attn_window_dev(const float* q, const void* kc, const void* vc, flo
     if (!(scale > 0.f) || !std::isfinite(scale)) return fail("attn_window: the scale is not a positive number");
     const size_t need = tm_cuda_attn_window_scratch(T, H, KVH, dh);
     if (scratch_bytes < need) return fail("attn_window: %zu bytes of scratch, %zu are needed", scratch_bytes, need);
+    if (overlap(q, (size_t)T * H * dh * 4, out, (size_t)T * H * dh * 4)) return fail("attn_window: out overlaps q");
     if (!on_library_device("attn_window")) return false;
     if (!T) return true;
     const KvBatch c{kc, vc, nullptr, nullptr, nullptr, 1, KVH, dh, ctx, 1, 1, T, ctx, pos0 + T, -1};

@@ -78,6 +78,7 @@ extern "C" bool tm_cuda_kv_append_paged_dev(const tm_cuda_kv_pages* kv, const fl
     if ((uintptr_t)qkv % 16 || (uintptr_t)q % 16 || (uintptr_t)rope % 16) return fail("kv_append_paged: qkv, q and rope lie on 16-byte boundaries");
     if (rope && !rope_rows) return fail("kv_append_paged: an empty rope table");
     if (rope_rows > 0x7fffffffu) rope_rows = 0x7fffffffu;
+    if (overlap(q, (size_t)T * H * c.dh * 4, qkv, (size_t)T * (H + 2 * (size_t)c.KVH) * c.dh * 4)) return fail("kv_append_paged: q overlaps qkv");
     if (!on_library_device("kv_append_paged")) return false;
     if (!T) return true;
     const dim3 grid(T, ((H + c.KVH) * (c.dh / 8) + c.KVH * c.dh / 4 + 255) / 256);

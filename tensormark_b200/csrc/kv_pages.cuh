@@ -119,5 +119,6 @@ constexpr float kLog2e = 1.4426950408889634f;
 // host side (attn_pages.cu): the checks that every entry over such a batch makes; that the library is up on the current device
 bool kv_batch_from(KvBatch* c, const tm_cuda_kv_pages* kv, unsigned T, unsigned H, const char* who);
 bool on_library_device(const char* who);
+inline bool overlap(const void* a, size_t na, const void* b, size_t nb) { return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na; }
 
 }  // namespace tmc

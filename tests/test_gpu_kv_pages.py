@@ -145,6 +145,46 @@ def test_long_and_ragged(cuda, torch_mod, half):
     Batch(torch_mod, [1] * 300, list(range(1, 301)), 4, 2, 64, 8, half, seed=5).check(cuda)
 
 
+@pytest.mark.parametrize("B,KVH,rep,dh,longest,window", [
+    (1, 8, 4, 128, 20000, 0), (1, 8, 4, 128, 3000, 0), (1, 1, 8, 64, 9000, 0), (1, 149, 1, 64, 130, 0), (2, 8, 4, 128, 400, 0), (5, 8, 2, 64, 900, 100),
+    (9, 8, 4, 128, 450, 0), (18, 8, 1, 64, 300, 0), (19, 8, 4, 128, 700, 60), (37, 8, 4, 64, 450, 0), (38, 8, 4, 64, 450, 0), (36, 8, 16, 128, 200, 0),
+])
+def test_around_one_launch_and_two(cuda, torch_mod, B, KVH, rep, dh, longest, window):
+    """Clusters of 16 CTAs down to one, and the list of tiles: a sequence of the longest length, others anywhere below it."""
+    rng = np.random.default_rng(B)
+    total = [longest] + rng.integers(1, longest + 1, B - 1).tolist()
+    for half in (True, False):
+        Batch(torch_mod, [1] * B, total, KVH * rep, KVH, dh, 16, half, seed=B).check(cuda, window, 3)
+
+
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("new,total,H,KVH,dh,window", [([5], [3000], 8, 2, 128, 0), ([9], [700], 4, 1, 64, 0), ([20], [1500], 4, 1, 128, 130), ([130], [900], 4, 1, 64, 0),
+                                                       ([66], [66], 8, 8, 128, 0), ([257, 64], [300, 1000], 4, 4, 64, 40), ([40, 1, 33, 1], [900, 200, 33, 1], 8, 2, 128, 500)])
+def test_shared_keys_of_a_chunk(cuda, torch_mod, new, total, H, KVH, dh, window, half):
+    """Tiles of rows whose keys one to eight CTAs share, some of them without a key."""
+    Batch(torch_mod, new, total, H, KVH, dh, 16, half, seed=new[0]).check(cuda, window, 5)
+
+
+def test_two_calls_at_once(cuda, torch_mod):
+    """Two batches on two streams at a time, each with scratch of its own."""
+    t = torch_mod
+    batches = [Batch(t, [1] * 30, list(range(100, 1600, 50)), 32, 8, 128, 16, True, seed=1), Batch(t, [200, 1], [900, 300], 8, 2, 64, 16, True, seed=2)]
+    streams, outs, keep = [t.cuda.Stream() for _ in batches], [], []
+    t.cuda.synchronize()
+    for b in batches:
+        need = cuda.tm_cuda_attn_paged_scratch(b.T, b.B, max(b.new), b.H, b.KVH, b.dh)
+        keep.append((t.empty(need // 4 + 1, device="cuda"), need))
+        outs.append(t.full((b.T, b.H * b.dh), 7.0, device="cuda"))
+    t.cuda.synchronize()
+    for _ in range(10):
+        for b, s, o, (scratch, need) in zip(batches, streams, outs, keep):
+            lib.check(cuda.tm_cuda_attn_paged_dev(C.byref(b.desc), ptr(b.d["q"]), ptr(scratch), need, ptr(o), b.T, max(b.new), b.H, 0, 0, 1 / np.sqrt(b.dh),
+                                                  C.c_void_p(s.cuda_stream)), "attn_paged")
+    t.cuda.synchronize()
+    for b, o in zip(batches, outs):
+        b.verify(o.cpu().numpy())
+
+
 @pytest.mark.parametrize("half", [True, False])
 def test_rows_that_see_nothing(cuda, torch_mod, half):
     """More new tokens than positions: those before position 0 give zeros. Rows of q and out behind the last sequence stay."""
@@ -376,3 +416,87 @@ def test_append_then_attend_captured(cuda, torch_mod):
         for s in range(3):
             want, tol = reference(qs[s].reshape(1, H, dh), *b.rows(s), b.total[s] - 1, 25, 2, 0.125)
             assert np.all(np.abs(got[s].reshape(1, H, dh) - want) <= tol)
+
+
+@pytest.mark.parametrize("half", [True, False])
+def test_serving_loop(cuda, torch_mod, half):
+    """Prompts in one chunk, then token by token: append, attention, logits, rules, choice, against the same in 64 bits on the tokens
+    that the GPU chose. The choice is checked where the two largest logits are further apart than the logits' tolerance."""
+    t, rng = torch_mod, np.random.default_rng(4)
+    H, KVH, dh, page, V, steps = 4, 2, 64, 16, 600, 12
+    W = (H + 2 * KVH) * dh
+    table_e = rng.standard_normal((V, W)).astype(np.float32)
+    head = (rng.standard_normal((H * dh, V)) / 16).astype(np.float32)
+    prompts = [rng.integers(0, V, n).tolist() for n in (37, 1, 90)]
+    B, cap = 3, 128
+    npages, ld = B * cap // page, cap // page
+    table = rng.permutation(npages).astype(np.int32).reshape(B, ld)
+    kind = t.float16 if half else t.float32
+    d = {"k": t.zeros(npages, KVH, page, dh, dtype=kind, device="cuda"), "v": t.zeros(npages, KVH, page, dh, dtype=kind, device="cuda"),
+         "table": t.from_numpy(table).cuda(), "q_begin": t.zeros(B + 1, dtype=t.int32, device="cuda"), "kv_len": t.zeros(B, dtype=t.int32, device="cuda")}
+    desc = lib.KvPages(B=B, KVH=KVH, dh=dh, page=page, npages=npages, table_ld=ld, kv_half=int(half), **{n: x.data_ptr() for n, x in d.items()})
+    rope = rope_table(cap, dh)
+    dr, dw, de = (t.from_numpy(x).cuda() for x in (rope, head, table_e))
+    lists = t.full((B, cap), -1, dtype=t.int32, device="cuda")
+    counts, prompt_n = t.zeros(B, dtype=t.int32, device="cuda"), t.tensor([len(p) for p in prompts], dtype=t.int32, device="cuda")
+    rep, pres, freq = (t.tensor(x, dtype=t.float32, device="cuda") for x in ([1.2, 1.5, 1.0], [0.1, 0.0, 0.3], [0.05, 0.2, 0.0]))
+    mask = rng.integers(0, 2 ** 32, (B, (V + 31) // 32), dtype=np.uint32)
+    dm = t.from_numpy(mask.view(np.int32)).cuda()
+    rules = lib.LogitRules(tokens=lists.data_ptr(), n_tokens=counts.data_ptr(), n_prompt=prompt_n.data_ptr(), tokens_ld=cap, repeat=rep.data_ptr(),
+                           presence=pres.data_ptr(), frequency=freq.data_ptr(), mask=dm.data_ptr(), mask_ld=mask.shape[1])
+    seqs, new = [list(p) for p in prompts], [list(p) for p in prompts]
+    bits = (mask[:, :, None] >> np.arange(32, dtype=np.uint32) & 1).reshape(B, -1)[:, :V].astype(bool)
+    sure = 0
+    for step in range(steps):
+        begin = np.concatenate([[0], np.cumsum([len(n) for n in new])]).astype(np.int32)
+        T, max_q = int(begin[-1]), max(len(n) for n in new)
+        d["q_begin"].copy_(t.from_numpy(begin)); d["kv_len"].copy_(t.tensor([len(s) for s in seqs], dtype=t.int32))
+        for b in range(B):
+            lists[b, :len(seqs[b])] = t.tensor(seqs[b], dtype=t.int32)
+        counts.copy_(d["kv_len"])
+        qkv = de[t.tensor(sum(new, []), device="cuda")].contiguous()
+        q, out = t.empty(T, H * dh, device="cuda"), t.empty(T, H * dh, device="cuda")
+        need = cuda.tm_cuda_attn_paged_scratch(T, B, max_q, H, KVH, dh)
+        scratch = t.empty(need // 4 + 1, device="cuda")
+        lib.check(cuda.tm_cuda_kv_append_paged_dev(C.byref(desc), ptr(qkv), ptr(q), T, H, ptr(dr), cap, stream_ptr(t)), "append")
+        lib.check(cuda.tm_cuda_attn_paged_dev(C.byref(desc), ptr(q), ptr(scratch), need, ptr(out), T, max_q, H, 48, 2, 0.125, stream_ptr(t)), "attention")
+        logits = (out[t.from_numpy(begin[1:] - 1).long().cuda()].double() @ dw.double()).float()
+        ruled, token = t.empty_like(logits), t.zeros(B, dtype=t.int32, device="cuda")
+        lib.check(cuda.tm_cuda_logits_rules_dev(ptr(logits), V, ptr(ruled), V, B, V, C.byref(rules), stream_ptr(t)), "rules")
+        for b in range(B):
+            lib.check(cuda.tm_cuda_argmax_dev(ptr(ruled[b]), ptr(token[b:]), V, stream_ptr(t)), "argmax")
+        t.cuda.synchronize()
+        assert cuda.tm_cuda_tok_flush()
+        got, chosen = ruled.cpu().numpy(), token.cpu().tolist()
+        for b in range(B):
+            x = table_e[seqs[b]].astype(np.float64).reshape(-1, H + 2 * KVH, dh)
+            c, sn = rope[:len(x), None, :, 0].astype(np.float64), rope[:len(x), None, :, 1].astype(np.float64)
+            lo, hi = x[:, :H + KVH, :dh // 2], x[:, :H + KVH, dh // 2:]
+            y = np.concatenate((lo * c - hi * sn, lo * sn + hi * c), 2)
+            kk, vv = y[:, H:], x[:, H + KVH:]
+            want, tol = reference(y[-1:, :H], kk, vv, len(x) - 1, 48, 2, 0.125)
+            # the caches' rounding: a key's half step moves a score by at most A 2^-11, a value's the result by size 2^-11; both through softmax
+            if half:
+                A = max(np.abs(kk[:, h // 2] @ y[-1, h]).max() + np.linalg.norm(y[-1, h]) * np.linalg.norm(kk[:, h // 2], axis=1).max() for h in range(H)) * 0.125
+                tol = tol + (2 * A + 1) * 2.0 ** -11 * np.abs(vv).max()
+            z = want.reshape(-1) @ head
+            ztol = tol.reshape(-1) @ np.abs(head) + np.abs(want.reshape(-1)) @ np.abs(head) * 2.0 ** -22
+            n, first = len(seqs[b]), len(prompts[b])
+            r, p, f = float(rep[b]), float(pres[b]), float(freq[b])
+            for tok in set(seqs[b]):
+                made = seqs[b][first:].count(tok)
+                z[tok] = (z[tok] / r if z[tok] > 0 else z[tok] * r) - f * made - p * (made > 0)
+                ztol[tok] *= max(1.0, r)
+            ztol = ztol + (np.abs(z) + 4) * 2.0 ** -22
+            assert np.isneginf(got[b][~bits[b]]).all()
+            assert np.all(np.abs(got[b] - z)[bits[b]] <= ztol[bits[b]]), (step, b)
+            z[~bits[b]] = -np.inf
+            best = int(np.argmax(z))
+            second = np.max(np.delete(z, best))
+            if z[best] - second > 2 * ztol.max():
+                assert chosen[b] == best
+                sure += 1
+            assert bits[b][chosen[b]]
+        new = [[c] for c in chosen]
+        seqs = [s + n for s, n in zip(seqs, new)]
+    assert half or sure > 25

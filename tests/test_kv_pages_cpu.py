@@ -41,7 +41,7 @@ BAD_PAGES = [(dict(k=None), "null"), (dict(v=None), "null"), (dict(table=None), 
 @pytest.mark.parametrize("kw,word", BAD_PAGES)
 def test_cache_descriptions(L, kw, word):
     kv = pages(**kw)
-    refused(L, L.tm_cuda_attn_paged_dev(C.byref(kv), A, A, 1 << 40, A, 5, 2, 8, 0, 0, 0.1, None), "attn_paged", word)
+    refused(L, L.tm_cuda_attn_paged_dev(C.byref(kv), A, A, 1 << 40, 2 * A, 5, 2, 8, 0, 0, 0.1, None), "attn_paged", word)
     refused(L, L.tm_cuda_kv_append_paged_dev(C.byref(kv), A, A, 5, 8, A, 100, None), "kv_append_paged", word)
 
 
@@ -54,6 +54,8 @@ def test_attention_arguments(L):
         refused(L, call(C.byref(kv), A, A, 1 << 40, A, 5, 2, 8, 0, 0, scale, None), "scale")
     refused(L, call(C.byref(kv), A, A, need - 1, A, 5, 2, 8, 0, 0, 0.1, None), "scratch")
     refused(L, call(C.byref(kv), A, A, 1 << 40, A, 1 << 31, 2, 8, 0, 0, 0.1, None), "2^31")
+    refused(L, call(C.byref(kv), A, A, 1 << 40, A, 5, 2, 8, 0, 0, 0.1, None), "overlaps")
+    refused(L, call(C.byref(kv), A + 5 * 8 * 64 * 4 - 16, A, 1 << 40, A, 5, 2, 8, 0, 0, 0.1, None), "overlaps")
     refused(L, call(None, A, A, 1 << 40, A, 5, 2, 8, 0, 0, 0.1, None), "null")
     refused(L, call(C.byref(kv), A, A, 1 << 40, A, 5, 2, 0, 0, 0, 0.1, None), "query heads")
     refused(L, call(C.byref(kv), A, A, 1 << 40, A, 5, 2, 2 * 129, 0, 0, 0.1, None), "query heads")
@@ -70,7 +72,7 @@ def test_window_arguments(L):
                      (dict(T=11), "positions"), (dict(T=5, pos0=6), "positions"), (dict(pos0=11, T=0), "positions"), (dict(pos0=2 ** 32 - 1, T=2), "positions"),
                      (dict(ctx=0, T=0), "positions"), (dict(ctx=1 << 31), "positions"), (dict(H=7), "query heads"), (dict(H=0), "query heads"),
                      (dict(KVH=0), "query heads"), (dict(H=2 * 130), "query heads"), (dict(dh=0), "head dimension"), (dict(dh=4), "head dimension"),
-                     (dict(dh=256), "head dimension"), (dict(n=need - 1), "scratch"), (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale")):
+                     (dict(dh=256), "head dimension"), (dict(n=need - 1), "scratch"), (dict(), "overlaps"), (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale")):
         refused(L, call(**kw), "attn_window", word)
 
 
@@ -81,6 +83,7 @@ def test_append_arguments(L):
     for x, q, r in ((A + 4, A, A), (A, A + 8, A), (A, A, A + 8)):
         refused(L, call(C.byref(kv), x, q, 5, 8, r, 9, None), "16-byte")
     refused(L, call(C.byref(kv), A, A, 5, 8, A, 0, None), "rope")
+    refused(L, call(C.byref(kv), A, A + 5 * 12 * 64 * 4 - 16, 5, 8, A, 9, None), "overlaps")
 
 
 def test_rules_arguments(L):
