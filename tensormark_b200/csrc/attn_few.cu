@@ -560,7 +560,27 @@ __global__ void __launch_bounds__(kMergeGroups * 128) attn_few_merge_kernel(cons
     const KvSeq s = kv_seq(a.c, (uint32_t)p.b);
     if (r >= s.n * a.rep) return;
     const uint32_t parts = (uint32_t)p.last - c + 2;
+    float* const to = a.out + ((size_t)(s.q0 + r / a.rep) * a.H + p.h * a.rep + r % a.rep) * dh + d;
     auto row_of = [&](uint32_t i) { return (size_t)(2 * (c + i) - (i ? 2 : 1)) * slot_rows + r; };      // i = 0: slot 1 of CTA c - 1; else slot 0 of CTA c + i - 1
+    if (parts <= BATCH) {                                   // a unit that two or three stretches share: a thread per dim, no waiting for others
+        if (grp || d >= dh) return;
+        float2 ml[BATCH];
+        float x[BATCH], M = -CUDART_INF_F, L = 0.f, o = 0.f;
+#pragma unroll
+        for (uint32_t i = 0; i < BATCH; ++i)
+            if (i < parts) { ml[i] = __ldcg(stat + row_of(i)); x[i] = __ldcg(part + row_of(i) * dh + d); }
+#pragma unroll
+        for (uint32_t i = 0; i < BATCH; ++i)
+            if (i < parts) M = fmaxf(M, ml[i].x);
+#pragma unroll
+        for (uint32_t i = 0; i < BATCH; ++i)
+            if (i < parts) {
+                const float w = ml[i].x == -CUDART_INF_F ? 0.f : pow2(ml[i].x - M);
+                o = fmaf(w, x[i], o); L = fmaf(w, ml[i].y, L);
+            }
+        *to = L == 0.f ? 0.f : o / L;
+        return;
+    }
     float v[BATCH];
     auto request = [&](uint32_t i0) {
 #pragma unroll
@@ -600,7 +620,7 @@ __global__ void __launch_bounds__(kMergeGroups * 128) attn_few_merge_kernel(cons
     o = 0.f;
 #pragma unroll
     for (uint32_t i = 0; i < G; ++i) o += so[i][d];
-    a.out[((size_t)(s.q0 + r / a.rep) * a.H + p.h * a.rep + r % a.rep) * dh + d] = L == 0.f ? 0.f : o / L;
+    *to = L == 0.f ? 0.f : o / L;
 }
 
 // How many clusters of 1, 2, 4, 8, 16 CTAs run at a time on the current device; nullptr (and the reason recorded) where that cannot be found out.

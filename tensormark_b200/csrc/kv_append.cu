@@ -25,7 +25,7 @@ __device__ __forceinline__ float turn_lo(float x, float y, float c, float s) { r
 __device__ __forceinline__ float turn_hi(float x, float y, float c, float s) { return fmaf(x, s, __fmul_rn(y, c)); }
 
 template <typename T>
-__global__ void __launch_bounds__(256) kv_append_kernel(KvBatch c, const float* qkv, float* q, uint32_t H, const float2* rope, uint32_t rope_rows,
+__global__ void __launch_bounds__(512) kv_append_kernel(KvBatch c, const float* qkv, float* q, uint32_t H, const float2* rope, uint32_t rope_rows,
                                                         int* status) {
     const uint32_t t = blockIdx.x, dh = c.dh, KVH = c.KVH, half = dh / 2, per = dh / 8, turned = (H + KVH) * per;
     const uint32_t e = blockIdx.y * blockDim.x + threadIdx.x, i = 4 * (e - turned), h = e / per, j = 4 * (e % per);
@@ -81,8 +81,10 @@ extern "C" bool tm_cuda_kv_append_paged_dev(const tm_cuda_kv_pages* kv, const fl
     if (overlap(q, (size_t)T * H * c.dh * 4, qkv, (size_t)T * (H + 2 * (size_t)c.KVH) * c.dh * 4)) return fail("kv_append_paged: q overlaps qkv");
     if (!on_library_device("kv_append_paged")) return false;
     if (!T) return true;
-    const dim3 grid(T, ((H + c.KVH) * (c.dh / 8) + c.KVH * c.dh / 4 + 255) / 256);
-    launch_overlapped(kv->kv_half ? kv_append_kernel<__half> : kv_append_kernel<float>, grid, dim3(256), 0, (cudaStream_t)stream, c, qkv, q, H, (const float2*)rope,
+    // A token's items in as few blocks as hold them, and those no larger than they need be: a token's sequence is looked for once per warp.
+    const unsigned items = (H + c.KVH) * (c.dh / 8) + c.KVH * c.dh / 4, blocks = (items + 511) / 512, threads = ((items + blocks - 1) / blocks + 31) / 32 * 32;
+    const dim3 grid(T, blocks);
+    launch_overlapped(kv->kv_half ? kv_append_kernel<__half> : kv_append_kernel<float>, grid, dim3(threads), 0, (cudaStream_t)stream, c, qkv, q, H, (const float2*)rope,
                       rope_rows, device_status_word());
     note_launch();
     return check_launch("kv_append_paged");
