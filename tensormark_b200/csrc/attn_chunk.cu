@@ -4,15 +4,23 @@
 // tiles of 128 keys that any of them sees: S = Q K^T, P = 2^(S - m), O = O corr + P V, with the running maximum m of each row.
 //
 // Bound: the tensor pipe. q and the weights are fp32 values as two fp16 parts each, high and low (error 2^-22, so that the result is as
-// good as fp32 products'), which doubles the products: for heads of 128 a tile of 128 x 128 takes 4 x 512 clocks, against 1024 for its
-// exponentials and about 1200 of the four schedulers' issue for the softmax and the output's update.
+// good as fp32 products'), which doubles the products: for heads of 128 both row tiles' products of a tile of keys take 4096 clocks.
+// A round of both takes some 6000: of a row tile's part 2000 are its own softmax (a warp per scheduler, latency and 32 exponentials per 4
+// clocks; with a row's maximum 600), the rest waits for the products of both. 2 x 1000 tokens over 15000 positions of 32 / 8 heads of
+// 128: 0.83 ms at first and 0.97 once the power cap has brought the clock down, when the 1002 GFLOP of the parts' products run at 0.75 of what
+// cuBLAS sustains in bf16. 1000 tokens with a window of 1024: 53 us, nine tiles of keys per CTA and some 10 us of beginning and end.
 //   * The two row tiles alternate: the products of one run while the other's softmax does. One barrier each way per tile: `done` says
 //     that S(j + 1) and P V(j) are there, `ready` that P(j) is and both of those have been taken.
 //   * P overwrites S in TMEM, 16 columns at a time: 8 of the high parts, 8 of the low ones. It is the A operand of the second product.
-//   * The output is summed in registers (a row per thread), tile by tile: a tensor core's own running sum is cut, not rounded, at every
-//     step, which over thousands of keys costs more than the parts' rounding; and the correction by the maximum is then one FMA.
-//   * K and V come by cp.async, one lane looking up the pages of four rows, into a ring of buffers in the order K, V, K, V. They are
-//     swizzled as they are written; V is the second product's B operand with its rows as the summed dimension.
+//   * Low parts are multiplied first: the tensor core cuts its running sum at every step, and a sum that is still small loses less
+//     (error 2.2e-6 with the parts in turn, 0.6e-6 so). For the same reason the output is summed in registers (a row per thread), tile by
+//     tile, which also makes the correction by the maximum one FMA. That is done while the exponentials of the next tile run.
+//   * K and V come by cp.async into a ring of buffers in the order K, V, K, V, one lane looking up the pages of four rows, and arrive on the
+//     buffer's barrier as they land; the issuing warp's proxy fence orders them before the products' reads. They are swizzled as they
+//     are written; V is the second product's B operand with its rows as the summed dimension.
+//   * Shared memory leaves no L1, so a spilled register costs a trip to L2: what a row's thread seldom needs waits in shared memory,
+//     tiles with hidden keys have S overwritten by a loop of its own, and the issuing warp walks its products in fours.
+//   * The keys of few row tiles are split over a cluster, whose CTAs put their rows into shared memory and merge a share each.
 //   * What is masked for one row but not for another meets a weight of 0, which is NaN if the value is not finite: a row whose result
 //     is not finite is computed again key by key, where masked keys are skipped.
 #include "attn_rows.cuh"
@@ -581,7 +589,8 @@ ChunkPlan plan_attn_chunk(uint32_t T, uint32_t B, uint32_t KVH, uint32_t rep, ui
     ChunkPlan pl;
     pl.slots = (uint32_t)(rows / row_tile + std::min<unsigned long long>(B, rows / (few + 1ull)));
     pl.splits = 1;
-    while (pl.splits < 8 && 2 * pl.splits * least * KVH <= 148) pl.splits *= 2;
+    const uint32_t ctas = row_tile == kChunkRows ? 148 : 296;           // that run at a time
+    while (pl.splits < 8 && 2 * pl.splits * least * KVH <= ctas) pl.splits *= 2;
     return pl;
 }
 

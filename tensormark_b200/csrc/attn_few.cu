@@ -2,16 +2,22 @@
 //
 // out = sum_j p_j v_j / sum_j p_j, p_j = 2^(s_j - m), s = scale log2(e) q k, with the running maximum m of one pass over the keys.
 //
-// Bound: HBM, every visible K and V row is read once for all the query rows of its head. The work of the whole batch - (sequence,
-// K/V head, tile of 64 keys), tiles in order - is one list of which every CTA takes an equal stretch, whatever the lengths are; a
-// CTA finishes the units that lie in its stretch and leaves a partial of the one or two that it shares, which a second kernel merges.
-//   * A warp takes 16 keys of every tile through a ring of its own (cp.async, one lane looks up one row's page), so nothing in the
+// Bound: HBM, every visible K and V row is read once for all the query rows of its head: 64 sequences of 150 to 8100 positions, 32 / 8 heads of
+// 128 in fp16, 1.10 GB in 185 us, 5.9 TB/s (0.91 of the copy rate); fp32 caches 4.4 TB/s. Short calls are bound by their trips to memory
+// one after the other (lengths, page, rows, merge): one token at 601 positions 7.0 us.
+//   * LIST: the work of the whole batch - (sequence, K/V head, tile of keys), tiles in order - is one list of which every CTA takes an
+//     equal stretch, whatever the lengths are; a CTA finishes the units that lie in its stretch and leaves a partial of the one or two that
+//     it shares, which a second kernel merges. Else, where the host can tell that few tiles are in reach, a unit is a cluster's, which
+//     merges through distributed shared memory in the same launch (one token at 601 positions 8.9 -> 7.0 us, 4096 keys of one 13.3 -> 11.4).
+//   * A warp takes 16 (8) keys of every tile through a ring of its own (cp.async, one lane looks up one row's page), so nothing in the
 //     loop waits for another warp.
 //   * Both products run on mma.sync with the query rows as its 16 rows: the keys' and values' bytes are the traffic, so the padding
 //     costs nothing that counts. Results are to be as good as fp32's, so an fp32 operand is two fp16 parts (two tf32 parts against
 //     fp32 caches), high and low: error 2^-22. With at most 8 rows the parts are the two halves of the 16 rows: one product.
 //     q is scaled by a power of two per row, and weights by 2^14, which keeps the low parts in fp16's normal range.
-//   * The output is summed in fp32 registers, 16 keys at a time: a tensor core's own running sum is cut, not rounded, at every step.
+//   * The output is summed in fp32 registers, a step's keys at a time: a tensor core's own running sum is cut, not rounded, at every step.
+//   * Over fp32 caches the same kernel takes longer chunks, 16 rows at a time (a.tiled): 700 tokens with a window of 255, 32 / 4 heads of 64,
+//     76 us, bound by the instructions that split K and V for every 16 rows.
 //   * A value that is masked for one row but not for another meets a weight of 0 in the product, which is NaN if the value is not
 //     finite. So a result that is not finite is computed again row by row, where masked keys are skipped.
 #include "attn_rows.cuh"
@@ -27,8 +33,9 @@
 namespace tmc {
 namespace {
 
-constexpr uint32_t kWarps = 4, kTile = 64, kStep = 16;      // keys of a tile; of a warp's share of it
-constexpr uint32_t kClusterTiles = 6;                       // one launch may walk so many tiles more than two would
+constexpr uint32_t kWarps = 4;                              // of a CTA; each takes its share of every tile
+// One launch may walk so many tiles more than two would: a tile takes some 0.6 us, the second launch 3 to 4.
+constexpr uint32_t kClusterTiles = 6;
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -61,7 +68,7 @@ __device__ __forceinline__ void parts(float x, uint32_t& hi, uint32_t& lo) {    
 }
 
 // ---- the list of work ------------------------------------------------------------------------------------------------
-struct Unit : KeyTiles<kTile> {
+template <uint32_t TILE> struct Unit : KeyTiles<TILE> {
     KvSeq s;
     bool bad;                       // its rows are NaN
 };
@@ -71,8 +78,8 @@ __device__ __forceinline__ uint32_t row_tiles(const AttnCall& a, uint32_t b, boo
     return s.n * a.rep <= a.few ? 0u : (s.n * a.rep + kFewRows - 1) / kFewRows;
 }
 // The rows of sequence b together (r0 = 0 and not more than `few`), or 16 of them from r0 on
-__device__ Unit unit_of(const AttnCall& a, uint32_t b, uint32_t r0) {
-    Unit u;
+template <uint32_t TILE> __device__ Unit<TILE> unit_of(const AttnCall& a, uint32_t b, uint32_t r0) {
+    Unit<TILE> u;
     u.s = kv_seq(a.c, b);
     u.bad = u.s.bad || u.s.n > a.max_q;
     if (a.tiled) {
@@ -87,14 +94,17 @@ __device__ Unit unit_of(const AttnCall& a, uint32_t b, uint32_t r0) {
 
 struct Part { int b, h, last, first; };     // of CTA c: the unit in whose middle its stretch begins, the CTA that ends it, whether c is the first that begins in it
 
+// Two CTAs per SM: 700 tokens of 32 / 4 heads of 64 in fp32 took 144 us with one (four stages), 84 with two (three). fp32 rows of 128 dims come
+// eight keys at a time for that: 32 sequences of 500 to 4000 positions, 32 / 8 heads, 240 us with 16 and one CTA, 138 so.
 template <typename T, int DHP, bool PAIR> struct Few {
+    static constexpr uint32_t Step = sizeof(T) == 4 && DHP == 128 ? 8 : 16, Tile = kWarps * Step;        // keys of a warp's share of a tile; of a tile
     static constexpr uint32_t Rows = PAIR ? 8 : 16;
-    static constexpr uint32_t RowBytes = DHP * sizeof(T), StageBytes = 2 * kStep * RowBytes;     // K and V of a warp's step
-    // two CTAs per SM where their rings fit: 700 tokens of 32 / 4 heads of 64 in fp32 take 144 us with one (four stages), 84 with two (three)
+    static constexpr uint32_t RowBytes = DHP * sizeof(T), StageBytes = 2 * Step * RowBytes;      // K and V of a warp's step
     static constexpr uint32_t Stages = sizeof(T) == 4 ? (DHP == 128 && !PAIR ? 2 : 3) : (PAIR ? 3 : 2) * (128 / DHP);
     static constexpr uint32_t Ring = kWarps * Stages * StageBytes, Merge = kWarps * Rows * DHP * 4;
     static constexpr uint32_t Smem = Ring + Merge;
-    static constexpr uint32_t PerSm = Smem <= 114688 ? 2 : 1;
+    static constexpr uint32_t PerSm = 2;
+    static_assert(Smem <= 114688, "two fit an SM");
 };
 
 // LIST: the stretches of the list. Else a unit per cluster of `splits` CTAs, which share its keys and merge through distributed shared
@@ -102,7 +112,9 @@ template <typename T, int DHP, bool PAIR> struct Few {
 template <typename T, int DHP, bool PAIR, bool LIST>
 __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_few_kernel(const __grid_constant__ AttnCall a, float* part, float2* stat, Part* meta, uint32_t splits) {
     using F = Few<T, DHP, PAIR>;
+    constexpr uint32_t kTile = F::Tile, kStep = F::Step, KB = kStep / 8;        // blocks of 8 keys of a step
     constexpr bool kHalf = sizeof(T) == 2;
+    static_assert(!kHalf || KB == 2);
     constexpr uint32_t RB = F::RowBytes, SB = F::StageBytes, S = F::Stages, ROWS = F::Rows, NB = DHP / 8, NR = PAIR ? 1 : 2;
     constexpr uint32_t KS = DHP / 16;                       // 16 dims at a time, whatever the type
     extern __shared__ __align__(128) uint8_t smem[];
@@ -119,7 +131,7 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
     unsigned long long x0, x1, total;
     uint32_t r0 = 0;                                        // a.tiled: the unit's first row
     const uint32_t split = LIST ? 0u : blockIdx.x % splits;
-    Unit u0;
+    Unit<kTile> u0;
     if constexpr (!LIST) {
         const uint32_t unit = (gridDim.x - 1 - blockIdx.x) / splits, slot = unit / KVH;
         uint32_t b = slot;
@@ -147,7 +159,7 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
             if (b == a.c.B) return;                         // the whole cluster
             r0 = at_t * kFewRows;
         }
-        u0 = unit_of(a, b, r0);
+        u0 = unit_of<kTile>(a, b, r0);
         if (u0.s.lost && at_h == 0 && tid == 0 && split == 0) note_bad_batch(a.status);
         if (u0.tiles == 0) return;
         x0 = (unsigned long long)u0.tiles * split / splits; x1 = (unsigned long long)u0.tiles * (split + 1) / splits;
@@ -158,7 +170,7 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
         const uint32_t per = (a.c.B + blockDim.x - 1) / blockDim.x, b0 = min(a.c.B, tid * per), b1 = min(a.c.B, b0 + per);
         unsigned long long mine = 0;
         for (uint32_t b = b0; b < b1; ++b) {
-            const Unit u = unit_of(a, b, 0);
+            const Unit<kTile> u = unit_of<kTile>(a, b, 0);
             if (u.s.lost && blockIdx.x == 0) note_bad_batch(a.status);
             mine += (unsigned long long)u.tiles * KVH;
         }
@@ -177,7 +189,7 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
         unsigned long long x = before + incl - mine;
         if (x0 >= x && x0 < x + mine) {                     // the stretch begins in one of this thread's sequences
             for (uint32_t b = b0; b < b1; ++b) {
-                const Unit u = unit_of(a, b, 0);
+                const Unit<kTile> u = unit_of<kTile>(a, b, 0);
                 const unsigned long long n = (unsigned long long)u.tiles * KVH;
                 if (x0 < x + n) {
                     const uint32_t h = (uint32_t)((x0 - x) / u.tiles), t = (uint32_t)((x0 - x) % u.tiles);
@@ -213,10 +225,10 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
     // ---- the copies: a cursor of their own, Stages - 1 tiles ahead ----
     uint32_t lb = at_b, lh = at_h, lt = at_t, left = (uint32_t)(x1 - x0), slot = 0;
     uint32_t no_page = 0;                                   // bit of a stage: a page was not there
-    Unit lu = !LIST ? u0 : unit_of(a, lb, 0);
+    Unit<kTile> lu = !LIST ? u0 : unit_of<kTile>(a, lb, 0);
     auto request = [&]() {
         if (left) {
-            const uint32_t place = lt * kTile + warp * kStep + (lane & 15u);
+            const uint32_t place = lt * kTile + warp * kStep + lane % kStep;
             size_t at = 0;
             const bool in = place < lu.count;
             bool ok = true;
@@ -243,7 +255,7 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
                 if (++lh == KVH) {
                     lh = 0;
                     lu.tiles = 0;
-                    while (lu.tiles == 0 && ++lb < a.c.B) lu = unit_of(a, lb, 0);
+                    while (lu.tiles == 0 && ++lb < a.c.B) lu = unit_of<kTile>(a, lb, 0);
                     if (lb >= a.c.B) left = 0;              // the arrays are not what they were: nothing behind them is read
                 }
             }
@@ -254,19 +266,19 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
 #pragma unroll
     for (uint32_t i = 0; i + 1 < S; ++i) request();
 
-    auto number_of = [&](const Unit& u, uint32_t h, uint32_t r) {        // of a row of a unit in q and out
+    auto number_of = [&](const Unit<kTile>& u, uint32_t h, uint32_t r) {        // of a row of a unit in q and out
         const uint32_t i = r / a.rep;
         return (size_t)(u.s.q0 + i) * a.H + h * a.rep + (r - i * a.rep);
     };
     // ---- the units of the stretch ----
     uint32_t b = at_b, h = at_h, t = at_t, todo = (uint32_t)(x1 - x0), use = 0, turn = 0;
-    Unit u = !LIST ? u0 : unit_of(a, b, 0);
+    Unit<kTile> u = !LIST ? u0 : unit_of<kTile>(a, b, 0);
     for (;;) {
         const uint32_t t0 = t, t1 = min(u.tiles, t + todo), rows = min(u.s.n * a.rep - r0, ROWS);
         int pos[NR];
         float back[NR], m[NR], l[NR], o[NB][2 * NR];        // back: what undoes q's power of two
         uint32_t qf[NR][KS][4];                             // fp16: the fragments, both parts; fp32: the values of a row, or their high parts
-        constexpr bool KEEP = !kHalf && DHP == 64;          // fp32: q's low parts are kept too, where registers are left
+        constexpr bool KEEP = !kHalf && (DHP == 64 || PAIR);  // fp32: q's low parts are kept too, where registers are left
         uint32_t qlow[KEEP ? NR : 1][KEEP ? KS : 1][4];
         {
             const float* qp[NR];
@@ -327,7 +339,7 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
             const uint32_t kat = ring + use * SB, vat = kat + kStep * RB, u0 = t * kTile + warp * kStep;        // the first place of this warp's step
             if (no_page >> use & 1u) lost_page = true;
             if (u0 < u.count) {
-                float s[2][4] = {}, low[2][4] = {};         // what the low parts add is summed apart: every step cuts the sum that it adds to
+                float s[KB][4] = {}, low[KB][4] = {};         // what the low parts add is summed apart: every step cuts the sum that it adds to
                 if constexpr (kHalf) {
                     const uint32_t key = (lane >> 4) * 8 + (lane & 7u), row = kat + key * RB, c0 = lane >> 3 & 1u;
 #pragma unroll
@@ -345,12 +357,15 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
                         for (uint32_t n = 0; n < NR; ++n) {
                             uint32_t h0 = qf[n][k / 2][2 * (k & 1)], h1 = qf[n][k / 2][2 * (k & 1) + 1], l0, l1;
                             if constexpr (KEEP) { l0 = qlow[n][k / 2][2 * (k & 1)]; l1 = qlow[n][k / 2][2 * (k & 1) + 1]; }
-                            else { parts(__uint_as_float(h0), h0, l0); parts(__uint_as_float(h1), h1, l1); }
+                            else {
+                                asm volatile("" : "+r"(h0), "+r"(h1));       // split here, at every tile: split once, outside, they would not fit the registers
+                                parts(__uint_as_float(h0), h0, l0); parts(__uint_as_float(h1), h1, l1);
+                            }
                             if constexpr (PAIR) { ah[0] = h0; ah[1] = l0; ah[2] = h1; ah[3] = l1; }
                             else { ah[n] = h0; al[n] = l0; ah[2 + n] = h1; al[2 + n] = l1; }
                         }
 #pragma unroll
-                        for (uint32_t nb = 0; nb < 2; ++nb) {
+                        for (uint32_t nb = 0; nb < KB; ++nb) {
                             const uint32_t key = nb * 8 + g, kx = (key & 3u) << 1 | (key >> 2 & 1u);
                             float2 f;
                             asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(f.x), "=f"(f.y) : "r"(kat + key * RB + (((2 * k + (t4 >> 1)) ^ kx) << 4) + (t4 & 1u) * 8));
@@ -364,25 +379,26 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
                 }
                 if constexpr (!kHalf || !PAIR) {
 #pragma unroll
-                    for (uint32_t i = 0; i < 8; ++i) s[i >> 2][i & 3] += low[i >> 2][i & 3];
+                    for (uint32_t i = 0; i < 4 * KB; ++i) s[i >> 2][i & 3] += low[i >> 2][i & 3];
                 }
                 const bool whole = u.seen(u0, kStep, p_least, from);
                 float corr[NR];
-                uint32_t ph[NR][4];                         // the weights as the second product's rows: PAIR: [0] both parts; else high, low
+                uint32_t ph[NR][2 * KB];                         // the weights as the second product's rows: PAIR: [0] both parts; else high, low
 #pragma unroll
                 for (uint32_t n = 0; n < NR; ++n) {
-                    float x[4];
+                    float x[2 * KB];
 #pragma unroll
-                    for (uint32_t i = 0; i < 4; ++i) {
+                    for (uint32_t i = 0; i < 2 * KB; ++i) {
                         if constexpr (PAIR) x[i] = (s[i >> 1][i & 1] + s[i >> 1][2 + (i & 1)]) * back[0];
                         else x[i] = s[i >> 1][2 * n + (i & 1)] * back[n];
                     }
                     if (!whole) {
 #pragma unroll
-                        for (uint32_t i = 0; i < 4; ++i)
+                        for (uint32_t i = 0; i < 2 * KB; ++i)
                             if (!kv_sees(a.mask, pos[n], (int)u.key(u0 + (i >> 1) * 8 + 2 * t4 + (i & 1)))) x[i] = -CUDART_INF_F;
                     }
-                    float mn = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                    float mn = fmaxf(x[0], x[1]);
+                    if constexpr (KB == 2) mn = fmaxf(mn, fmaxf(x[2], x[3]));
                     mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 1));
                     mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 2));
                     mn = fmaxf(mn, m[n]);
@@ -390,14 +406,16 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
                     corr[n] = pow2(m[n] - base);
                     m[n] = mn;
 #pragma unroll
-                    for (uint32_t i = 0; i < 4; ++i) x[i] = pow2(x[i] - base + kUp);
-                    l[n] = fmaf(l[n], corr[n], (x[0] + x[1]) + (x[2] + x[3]));
+                    for (uint32_t i = 0; i < 2 * KB; ++i) x[i] = pow2(x[i] - base + kUp);
+                    float add = x[0] + x[1];
+                    if constexpr (KB == 2) add += x[2] + x[3];
+                    l[n] = fmaf(l[n], corr[n], add);
                     if constexpr (kHalf) {
                         if constexpr (PAIR) { parts(x[0], x[1], ph[0][0], ph[0][1]); parts(x[2], x[3], ph[0][2], ph[0][3]); }
                         else { parts(x[0], x[1], ph[0][n], ph[NR - 1][n]); parts(x[2], x[3], ph[0][2 + n], ph[NR - 1][2 + n]); }
                     } else {
 #pragma unroll
-                        for (uint32_t i = 0; i < 4; ++i) ph[n][i] = __float_as_uint(x[i]);
+                        for (uint32_t i = 0; i < 2 * KB; ++i) ph[n][i] = __float_as_uint(x[i]);
                     }
                 }
                 if constexpr (kHalf) {
@@ -420,9 +438,9 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
                         }
                     }
                 } else {
-                    uint32_t ah[2][4], al[2][4];            // key 2 t of a block of 8 is row t of the product's operand, key 2 t + 1 row t + 4
+                    uint32_t ah[KB][4], al[KB][4];            // key 2 t of a block of 8 is row t of the product's operand, key 2 t + 1 row t + 4
 #pragma unroll
-                    for (uint32_t nb = 0; nb < 2; ++nb)
+                    for (uint32_t nb = 0; nb < KB; ++nb)
 #pragma unroll
                         for (uint32_t n = 0; n < NR; ++n) {
                             uint32_t h0, l0, h1, l1;
@@ -435,7 +453,7 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
                     for (uint32_t i = 0; i < NB; ++i) {
                         float d[4] = {};
 #pragma unroll
-                        for (uint32_t nb = 0; nb < 2; ++nb) {
+                        for (uint32_t nb = 0; nb < KB; ++nb) {
                             uint32_t vh[2], vl[2];
 #pragma unroll
                             for (uint32_t k = 0; k < 2; ++k) {
@@ -506,7 +524,7 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
         if (__syncthreads_or(again && !bad)) {
             for (uint32_t r = warp; r < rows; r += kWarps) {
                 const size_t row = number_of(u, h, r0 + r);
-                row_again<T>(a, b, h, u.s.first + (int)((r0 + r) / a.rep), u, t0, t1, a.q + row * dh, all ? a.out + row * dh : po + (size_t)r * dh, all ? nullptr : ps + r);
+                row_again<T, kTile>(a, b, h, u.s.first + (int)((r0 + r) / a.rep), u, t0, t1, a.q + row * dh, all ? a.out + row * dh : po + (size_t)r * dh, all ? nullptr : ps + r);
             }
             if (!LIST) __syncthreads();
         }
@@ -538,7 +556,7 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
         if (++h == KVH) {
             h = 0;
             u.tiles = 0;
-            while (u.tiles == 0 && ++b < a.c.B) u = unit_of(a, b, 0);
+            while (u.tiles == 0 && ++b < a.c.B) u = unit_of<kTile>(a, b, 0);
             if (b >= a.c.B) return;
         }
     }
@@ -659,7 +677,7 @@ bool go(const AttnCall& a, float* scratch, cudaStream_t st) {
     const unsigned most = std::min(kFewCtas, (unsigned)device_sm_count() * F::PerSm);
     // the keys that a sequence can have in reach, as far as the host knows
     const unsigned long long keys = a.c.table ? a.c.cap : a.c.total, seen = (unsigned long long)a.mask.window + a.mask.sinks + a.max_q;
-    const unsigned long long each = ((a.mask.window && seen < keys ? seen + 2 * kTile : keys) + kTile - 1) / kTile, units = (unsigned long long)a.c.B * a.c.KVH, tiles = units * each;
+    const unsigned long long each = ((a.mask.window && seen < keys ? seen : keys) + F::Tile - 1) / F::Tile, units = (unsigned long long)a.c.B * a.c.KVH, tiles = units * each;
     int cs = 4;
     while (cs && ((units << cs) > most || fits->clusters[cs] < (int)units || (1ull << cs) >= 2 * each)) --cs;
     // of several sequences some may be short, which evens out over a list and not over clusters

@@ -69,6 +69,7 @@ bool tm_cuda_attn_paged_dev(const tm_cuda_kv_pages* kv, const float* q, float* s
                             unsigned H, unsigned window, unsigned sinks, float scale, void* stream) {
     KvBatch c;
     if (!kv_batch_from(&c, kv, T, H, "attn_paged")) return false;
+    if (!T) return true;
     if (!q || !out || !scratch) return fail("attn_paged: null pointer");
     if ((uintptr_t)q % 16 || (uintptr_t)out % 16 || (uintptr_t)scratch % 16) return fail("attn_paged: q, out and scratch lie on 16-byte boundaries");
     if (!(scale > 0.f) || !std::isfinite(scale)) return fail("attn_paged: the scale is not a positive number");
@@ -76,17 +77,17 @@ bool tm_cuda_attn_paged_dev(const tm_cuda_kv_pages* kv, const float* q, float* s
     if (scratch_bytes < need) return fail("attn_paged: %zu bytes of scratch, %zu are needed", scratch_bytes, need);
     if (overlap(q, (size_t)T * H * c.dh * 4, out, (size_t)T * H * c.dh * 4)) return fail("attn_paged: out overlaps q");
     if (!on_library_device("attn_paged")) return false;
-    if (!T) return true;
     return launch(AttnCall{c, kv_mask(window, sinks), q, out, H, H / c.KVH, max_q && max_q < T ? max_q : T, 0, false, scale, nullptr, false}, kv->kv_half != 0, scratch, (cudaStream_t)stream);
 }
 
 bool tm_cuda_attn_window_dev(const float* q, const void* kc, const void* vc, float* scratch, size_t scratch_bytes, float* out, unsigned T,
                              unsigned pos0, unsigned H, unsigned KVH, unsigned dh, unsigned ctx, unsigned window, unsigned sinks, float scale,
                              int kv_half, void* stream) {
-    if (!q || !kc || !vc || !scratch || !out) return fail("attn_window: null pointer");
     if (!KVH || !H || H % KVH || H / KVH > 128) return fail("attn_window: %u query heads for %u K/V heads (a multiple, at most 128 each)", H, KVH);
     if (!dh || dh % 8 || dh > 128) return fail("attn_window: head dimension %u (multiples of 8 up to 128)", dh);
     if (!ctx || ctx > 0x7fffff00u || pos0 > ctx || T > ctx - pos0) return fail("attn_window: positions %u to %llu of a cache of %u rows", pos0, (unsigned long long)pos0 + T, ctx);
+    if (!T) return true;
+    if (!q || !kc || !vc || !scratch || !out) return fail("attn_window: null pointer");
     if ((unsigned long long)T * H > 0x7fffffffull) return fail("attn_window: 2^31 query rows");
     if (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc | (uintptr_t)scratch | (uintptr_t)out) % 16) return fail("attn_window: q, the caches, scratch and out lie on 16-byte boundaries");
     if (!(scale > 0.f) || !std::isfinite(scale)) return fail("attn_window: the scale is not a positive number");
@@ -94,7 +95,6 @@ bool tm_cuda_attn_window_dev(const float* q, const void* kc, const void* vc, flo
     if (scratch_bytes < need) return fail("attn_window: %zu bytes of scratch, %zu are needed", scratch_bytes, need);
     if (overlap(q, (size_t)T * H * dh * 4, out, (size_t)T * H * dh * 4)) return fail("attn_window: out overlaps q");
     if (!on_library_device("attn_window")) return false;
-    if (!T) return true;
     const KvBatch c{kc, vc, nullptr, nullptr, nullptr, 1, KVH, dh, ctx, 1, 1, T, ctx, pos0 + T, -1};
     return launch(AttnCall{c, kv_mask(window, sinks), q, out, H, H / KVH, T, 0, false, scale, nullptr, false}, kv_half != 0, scratch, (cudaStream_t)stream);
 }

@@ -98,6 +98,15 @@ def test_rules_arguments(L):
     refused(L, L.tm_cuda_logits_rules_dev(A, 9, A, 9, 1, 9, None, None), "null")
 
 
+def test_nothing_to_do(L):
+    """No tokens, no rows: a call that does nothing, with the null pointers that empty tensors have."""
+    kv = pages()
+    assert L.tm_cuda_attn_paged_dev(C.byref(kv), None, None, 0, None, 0, 0, 8, 0, 0, 0.1, None)
+    assert L.tm_cuda_kv_append_paged_dev(C.byref(kv), None, None, 0, 8, None, 0, None)
+    assert L.tm_cuda_attn_window_dev(None, None, None, None, 0, None, 0, 10, 8, 2, 64, 10, 0, 0, 0.1, 1, None)
+    assert L.tm_cuda_logits_rules_dev(None, 100, None, 100, 0, 100, None, None)
+
+
 SRC = r"""
 #include "kv_pages.cuh"
 using namespace tmc;
