@@ -29,7 +29,7 @@ struct KvBatch {
     uint32_t total;             // without a table: positions in the cache
     int page_shift;             // log2(page), or -1
 };
-constexpr int kStatusBatch = 2;
+constexpr int kStatusBatch = 64;                // waits that run out have 1 and 2
 
 struct KvSeq {
     uint32_t q0, n;             // its rows of q and out; none where q_begin does not give a range of them
