@@ -141,18 +141,20 @@ __device__ __forceinline__ void parts(float x, float y, uint32_t& hi, uint32_t& 
 // Is key j hidden from position p, whose window begins at lo?
 __device__ __forceinline__ bool hidden(int j, int p, int lo, int sinks) { return (j > p) | ((j < lo) & (j >= sinks)); }
 
-// mbar_wait without a call in it: a row's 128 sums are live across most of these waits, more than a call may keep in registers
+// mbar_wait without a call in it (a row's 128 sums are live across most of these waits, more than a call may keep in registers), by a whole
+// warp, which leaves it together
 __device__ __forceinline__ bool wait_for(uint64_t& bar, uint32_t parity, volatile int* gone) {
     const uint32_t at = smem_u32(&bar);
-    if (mbar_test(at, parity) || mbar_try_wait(at, parity)) return true;
-    const unsigned long long t0 = global_ns();
-    for (uint32_t i = 1;; ++i) {
-        if (mbar_try_wait(at, parity)) return true;
-        if (i % 64 == 0) {
-            if (*gone) return false;
-            if (global_ns() - t0 > kWaitLimitNs) { *gone = 1; return false; }
-        }
+    bool there = mbar_test(at, parity) || mbar_try_wait(at, parity);
+    if (!there) {
+        const unsigned long long t0 = global_ns();
+        for (uint32_t i = 1; !(there = mbar_try_wait(at, parity)); ++i)
+            if (i % 64 == 0) {
+                if (*gone) break;
+                if (global_ns() - t0 > kWaitLimitNs) { *gone = 1; break; }
+            }
     }
+    return __all_sync(0xffffffffu, there);
 }
 
 struct Bars { uint64_t full[6], empty[6], ready[2], done[2]; };
@@ -172,8 +174,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
     const uint32_t dh = a.c.dh;
     pdl_enter();
 
-    // ---- which sequence, and which of its row tiles: counted from the last one (the longest of a prompt) ----
-    const uint32_t unit = (gridDim.x - 1 - blockIdx.x) / splits, slot = unit / a.c.KVH, h = unit % a.c.KVH, split = blockIdx.x % splits;
+    // ---- which sequence, and which of its row tiles: counted from the last one (the longest of a prompt). The host knows how many there are
+    // at most; CTAs beyond that come last and leave at once ----
+    const uint32_t unit = blockIdx.x / splits, h = unit % a.c.KVH, split = blockIdx.x % splits;
     auto slots_of = [&](uint32_t b, bool note) {
         const KvSeq s = kv_seq(a.c, b);
         if (s.lost && note) note_bad_batch(a.status);
@@ -182,10 +185,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
     };
     if (tid == 0) { unit_b = 0xffffffffu; gone = 0; bad_page = 0; }
     if (tid < 2 * kRows / 32) odd[tid] = 0;
-    if (a.c.B == 1) {
-        if (tid == 0 && slot < slots_of(0, true)) { unit_b = 0; unit_tile = slot; }
-        __syncthreads();
-    } else {
+    {
         const uint32_t per = (a.c.B + kThreads - 1) / kThreads, b0 = min(a.c.B, tid * per), b1 = min(a.c.B, b0 + per);
         uint32_t mine = 0;
         for (uint32_t b = b0; b < b1; ++b) mine += slots_of(b, blockIdx.x == 0);
@@ -194,8 +194,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
         for (int o = 1; o < 32; o <<= 1) { const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= (uint32_t)o) incl += y; }
         if (lane == 31) sums[warp] = incl;
         __syncthreads();
-        uint32_t before = incl - mine;
-        for (uint32_t w = 0; w < warp; ++w) before += sums[w];
+        uint32_t before = incl - mine, total = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < kThreads / 32; ++w) { if (w == warp) before += total; total += sums[w]; }
+        const uint32_t slot = total - 1 - unit / a.c.KVH;                // wraps where there is no such unit
         if (slot >= before && slot < before + mine)
             for (uint32_t b = b0; b < b1; ++b) {
                 const uint32_t n = slots_of(b, false);
@@ -266,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
             };
             ok = wait_full(0);
             for (uint32_t w = 0; w < tiles2 && ok; ++w) {
-                ok = wait_for(bars.ready[w], 0, &gone);      // q is there
+                ok = wait_for(bars.ready[w], 0, &gone);                  // q is there
                 if (!ok) break;
                 fence_after();
                 scores(w, 0);

@@ -133,8 +133,8 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
     const uint32_t split = LIST ? 0u : blockIdx.x % splits;
     Unit<kTile> u0;
     if constexpr (!LIST) {
-        const uint32_t unit = (gridDim.x - 1 - blockIdx.x) / splits, slot = unit / KVH;
-        uint32_t b = slot;
+        const uint32_t unit = blockIdx.x / splits;
+        uint32_t b = unit / KVH;
         if (tid == 0) { at_h = unit % KVH; sm_bad[0] = sm_bad[1] = 0; }
         if (a.tiled) {
             if (tid == 0) at_b = a.c.B;
@@ -146,8 +146,10 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
             for (int o = 1; o < 32; o <<= 1) { const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= (uint32_t)o) incl += y; }
             if (lane == 31) sums[warp] = incl;
             __syncthreads();
-            uint32_t before = incl - mine;
-            for (uint32_t w = 0; w < warp; ++w) before += (uint32_t)sums[w];
+            uint32_t before = incl - mine, all = 0;
+#pragma unroll
+            for (uint32_t w = 0; w < kWarps; ++w) { if (w == warp) before += all; all += (uint32_t)sums[w]; }
+            const uint32_t slot = all - 1 - unit / KVH;     // from the last on; wraps where there is no such unit
             if (slot >= before && slot < before + mine)
                 for (uint32_t i = b0; i < b1; ++i) {
                     const uint32_t n = row_tiles(a, i, false);

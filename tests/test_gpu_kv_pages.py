@@ -165,6 +165,14 @@ def test_shared_keys_of_a_chunk(cuda, torch_mod, new, total, H, KVH, dh, window,
     Batch(torch_mod, new, total, H, KVH, dh, 16, half, seed=new[0]).check(cuda, window, 5)
 
 
+@pytest.mark.parametrize("half", [True, False])
+def test_many_sequences_beside_chunks(cuda, torch_mod, half):
+    """A batch of which most decode: the CTAs for chunks that might have been there find none."""
+    new = [1] * 150 + [70] + [0] * 40 + [300] + [2] * 120
+    total = [n + (37 * i) % 200 for i, n in enumerate(new)]
+    Batch(torch_mod, new, total, 8, 2, 64, 16, half, seed=21).check(cuda, 90, 4)
+
+
 def test_two_calls_at_once(cuda, torch_mod):
     """Two batches on two streams at a time, each with scratch of its own."""
     t = torch_mod
