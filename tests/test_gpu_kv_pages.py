@@ -173,6 +173,133 @@ def test_many_sequences_beside_chunks(cuda, torch_mod, half):
     Batch(torch_mod, new, total, 8, 2, 64, 16, half, seed=21).check(cuda, 90, 4)
 
 
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("new,total,window", [([1] * 60, None, 0), ([1], [5000], 0), ([5, 1], [3000, 40], 700), ([300, 1], [900, 77], 0)])
+def test_scratch_is_enough(cuda, torch_mod, new, total, window, half):
+    """Nothing is written behind the scratch that was asked for, nor behind out or before it."""
+    t = torch_mod
+    total = total or [100 + 53 * i for i in range(len(new))]
+    b = Batch(t, new, total, 8, 2, 128, 16, half, seed=31)
+    need = cuda.tm_cuda_attn_paged_scratch(b.T, b.B, max(new), b.H, b.KVH, b.dh)
+    assert need % 16 == 0
+    scratch, out = t.full((need // 4 + 64,), 3.0, device="cuda"), t.full((b.T + 2, b.H * b.dh), 7.0, device="cuda")
+    lib.check(cuda.tm_cuda_attn_paged_dev(C.byref(b.desc), ptr(b.d["q"]), ptr(scratch), need, ptr(out[1:]), b.T, max(new), b.H, window, 2, 1 / np.sqrt(128),
+                                          stream_ptr(t)), "attn_paged")
+    t.cuda.synchronize()
+    assert bool((scratch[need // 4:] == 3.0).all()) and bool((out[0] == 7.0).all()) and bool((out[-1] == 7.0).all())
+    b.verify(out[1:-1].cpu().numpy(), window, 2)
+
+
+@pytest.mark.parametrize("half", [True, False])
+def test_offsets_past_32_bits(cuda, torch_mod, half):
+    """A cache of more than 2^32 elements: pages at both of its ends, written by append and read by attention, single tokens and a chunk."""
+    t, rng = torch_mod, np.random.default_rng(6)
+    H, KVH, dh, page = 8, 2, 128, 16
+    npages = 2 ** 32 // (KVH * page * dh) + 40
+    kind = t.float16 if half else t.float32
+    k, v = (t.empty(npages, KVH, page, dh, dtype=kind, device="cuda") for _ in range(2))
+    total, new = [90, 60, 33], [90, 60, 33]
+    table = np.full((3, 7), -1, np.int32)
+    table[0, :6] = npages - 1 - np.arange(6)
+    table[1, :4] = [0, npages - 30, 1, npages - 20]
+    table[2, :3] = [npages - 10, npages // 2 + 1, 5]
+    begin = np.array([0, 90, 150, 183], np.int32)
+    qkv = rng.standard_normal((183, (H + 2 * KVH) * dh)).astype(np.float32)
+    d = {"table": t.from_numpy(table).cuda(), "q_begin": t.from_numpy(begin).cuda(), "kv_len": t.tensor(total, dtype=t.int32, device="cuda")}
+    desc = lib.KvPages(k=k.data_ptr(), v=v.data_ptr(), B=3, KVH=KVH, dh=dh, page=page, npages=npages, table_ld=7, kv_half=int(half), **{n: x.data_ptr() for n, x in d.items()})
+    dq, q, out = t.from_numpy(qkv).cuda(), t.empty(183, H * dh, device="cuda"), t.empty(183, H * dh, device="cuda")
+    lib.check(cuda.tm_cuda_kv_append_paged_dev(C.byref(desc), ptr(dq), ptr(q), 183, H, None, 0, stream_ptr(t)), "append")
+
+    def attend(T, max_q, rows):
+        need = cuda.tm_cuda_attn_paged_scratch(T, 3, max_q, H, KVH, dh)
+        scratch = t.empty(need // 4 + 1, device="cuda")
+        lib.check(cuda.tm_cuda_attn_paged_dev(C.byref(desc), ptr(rows), ptr(scratch), need, ptr(out), T, max_q, H, 0, 0, 1 / np.sqrt(dh), stream_ptr(t)), "attention")
+        t.cuda.synchronize()
+        assert cuda.tm_cuda_tok_flush()
+        return out.cpu().numpy()
+
+    got = attend(183, 90, q)
+    x = qkv.reshape(-1, H + 2 * KVH, dh)
+    held = lambda a: a.astype(np.float16).astype(np.float32) if half else a  # noqa: E731
+    for b in range(3):
+        r = slice(begin[b], begin[b + 1])
+        want, tol = reference(x[r, :H], held(x[r, H:H + KVH]), held(x[r, H + KVH:]), 0, 0, 0, 1 / np.sqrt(dh))
+        assert np.all(np.abs(got[r].reshape(-1, H, dh) - want) <= tol)
+    d["q_begin"].copy_(t.arange(4, dtype=t.int32))                          # the last token of each again, as a decode step
+    got = attend(3, 1, q[t.from_numpy(begin[1:] - 1).long().cuda()].contiguous())
+    for b in range(3):
+        r = slice(begin[b], begin[b + 1])
+        want, tol = reference(x[r, :H][-1:], held(x[r, H:H + KVH]), held(x[r, H + KVH:]), total[b] - 1, 0, 0, 1 / np.sqrt(dh))
+        assert np.all(np.abs(got[b].reshape(1, H, dh) - want) <= tol)
+    del k, v
+    t.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("T", [1, 40])
+def test_far_into_a_long_contiguous_cache(cuda, torch_mod, T):
+    t, rng = torch_mod, np.random.default_rng(7)
+    KVH, H, dh, ctx = 8, 16, 64, 4_300_000                                   # 2.2e9 elements
+    first = ctx - 60
+    k, v = (t.empty(KVH, ctx, dh, dtype=t.float16, device="cuda") for _ in range(2))
+    near = {n: rng.standard_normal((KVH, 300, dh)).astype(np.float16) for n in "kv"}
+    sink = {n: rng.standard_normal((KVH, 3, dh)).astype(np.float16) for n in "kv"}
+    for n, c in (("k", k), ("v", v)):
+        c[:, ctx - 300:] = t.from_numpy(near[n]).cuda()
+        c[:, :3] = t.from_numpy(sink[n]).cuda()
+    q = rng.standard_normal((T, H * dh)).astype(np.float32)
+    dq, out = t.from_numpy(q).cuda(), t.empty(T, H * dh, device="cuda")
+    need = cuda.tm_cuda_attn_window_scratch(T, H, KVH, dh)
+    scratch = t.empty(need // 4 + 1, device="cuda")
+    lib.check(cuda.tm_cuda_attn_window_dev(ptr(dq), ptr(k), ptr(v), ptr(scratch), need, ptr(out), T, first, H, KVH, dh, ctx, 200, 3, 0.125, 1, stream_ptr(t)), "window")
+    t.cuda.synchronize()
+    got = out.cpu().numpy().reshape(T, H, dh)
+    for i in range(T):                                                      # the keys that token i sees, at positions of their own
+        p = first + i
+        lo = p - 199 - (ctx - 300)
+        kk, vv = (np.concatenate((sink[n], near[n][:, lo:p + 1 - (ctx - 300)]), 1).transpose(1, 0, 2) for n in "kv")
+        want, tol = reference(q[i].reshape(1, H, dh), kk, vv, len(kk) - 1, 0, 0, 0.125)
+        assert np.all(np.abs(got[i:i + 1] - want) <= tol)
+    del k, v, c
+    t.cuda.empty_cache()
+
+
+def test_graphs_that_share_scratch(cuda, torch_mod):
+    """Two captured graphs with one scratch, replayed in turn, while lengths and ranges of rows change between replays: sequences come and go."""
+    t = torch_mod
+    b = Batch(t, [1] * 40, [200 + 9 * i for i in range(40)], 8, 2, 128, 16, True, seed=41)
+    need = cuda.tm_cuda_attn_paged_scratch(b.T, b.B, 1, b.H, b.KVH, b.dh)
+    scratch, outs, graphs = t.empty(need // 4 + 1, device="cuda"), [], []
+    side = t.cuda.Stream()
+
+    def call(out, window, s):
+        lib.check(cuda.tm_cuda_attn_paged_dev(C.byref(b.desc), ptr(b.d["q"]), ptr(scratch), need, ptr(out), b.T, 1, b.H, window, 2, 1 / np.sqrt(128), s), "attention")
+
+    for window in (0, 90):
+        out = t.full((b.T, b.H * b.dh), 7.0, device="cuda")
+        with t.cuda.stream(side):
+            call(out, window, stream_ptr(t))
+        side.synchronize()
+        g = t.cuda.CUDAGraph()
+        with t.cuda.graph(g):
+            call(out, window, stream_ptr(t))
+        outs.append(out); graphs.append(g)
+    lengths = list(b.total)
+    for turn in range(4):
+        here = [int((i + turn) % 3 != 0) for i in range(40)]                # one new token, or none
+        b.new, b.total = here, [n - 30 * turn for n in lengths]
+        b.begin = np.concatenate([[0], np.cumsum(here)]).astype(np.int32)
+        b.d["q_begin"].copy_(t.from_numpy(b.begin)); b.d["kv_len"].copy_(t.tensor(b.total, dtype=t.int32))
+        for out in outs:
+            out.fill_(7.0)
+        for g in graphs + graphs[::-1]:
+            g.replay()
+        t.cuda.synchronize()
+        for out, window in zip(outs, (0, 90)):
+            got = out.cpu().numpy()
+            b.verify(got, window, 2)
+            assert np.all(got[b.begin[-1]:] == 7.0)
+
+
 def test_two_calls_at_once(cuda, torch_mod):
     """Two batches on two streams at a time, each with scratch of its own."""
     t = torch_mod

@@ -148,6 +148,28 @@ def test_same_id_twice_and_special_values(cuda, torch_mod):
     assert np.isneginf(run(cuda, torch_mod, x, 300, a)).all()
 
 
+def test_rows_far_apart(cuda, torch_mod):
+    """Strides whose products pass 32 bits."""
+    t, rng = torch_mod, np.random.default_rng(9)
+    V, ld = 5001, 1_500_000_003
+    x, a = case(rng, 3, V, 30, 4, True, V)
+    far = t.empty(2 * ld + V, dtype=t.float32, device="cuda")
+    for b in range(3):
+        far[b * ld:b * ld + V] = t.from_numpy(x[b]).cuda()
+    d = {n: t.from_numpy(v.view(np.int32) if v.dtype == np.uint32 else v).cuda() for n, v in a.items()}
+    r = lib.LogitRules(tokens_ld=30, bias_ld=4, mask_ld=a["mask"].shape[1], **{n: v.data_ptr() for n, v in d.items()})
+    lib.check(cuda.tm_cuda_logits_rules_dev(ptr(far), ld, ptr(far), ld, 3, V, C.byref(r), stream_ptr(t)), "logits_rules")
+    t.cuda.synchronize()
+    want, tol = plain(x, V, **a)
+    for b in range(3):
+        got = far[b * ld:b * ld + V].cpu().numpy().astype(np.float64)
+        same = ~np.isfinite(want[b])
+        with np.errstate(invalid="ignore"):
+            assert np.array_equal(got[same], want[b][same]) and np.all((np.abs(got - want[b]) <= tol[b]) | same)
+    del far
+    t.cuda.empty_cache()
+
+
 def test_a_step_to_the_token(cuda, torch_mod):
     """Rules, then the framework's choice: the token that the plain rules' largest logit has, lowest index on ties."""
     t, rng = torch_mod, np.random.default_rng(3)
