@@ -43,6 +43,9 @@ template <int DHP> struct Chunk {
     static constexpr uint32_t Tile = kKeys * DHP * 2;      // bytes of a tile of keys, or of one part of q; 64 dims are 128 bytes
     static constexpr uint32_t Half = kKeys * 128;
     static constexpr uint32_t Buffers = DHP == 128 ? 3 : 6;
+    // Heads of 64: the products of 64 keys' weights begin while the other 64 are worked out, O having taken all of the tile before by then (a mixed
+    // batch 40.8 -> 38.6 us). Heads of 128 would have to take twice as much in that time, and gain nothing.
+    static constexpr bool Early = DHP == 64;
     // registers of the warps that issue and of those that hold rows: of the 384 x 168 that the block is launched with
     static constexpr uint32_t RegsIssue = DHP == 128 ? 56 : 104, RegsRows = DHP == 128 ? 224 : 200;
     static_assert(RegsIssue + 2 * RegsRows <= 3 * 168);
@@ -157,7 +160,7 @@ __device__ __forceinline__ bool wait_for(uint64_t& bar, uint32_t parity, volatil
     return __all_sync(0xffffffffu, there);
 }
 
-struct Bars { uint64_t full[6], empty[6], ready[2], done[2]; };
+struct Bars { uint64_t full[6], empty[6], half[2], ready[2], done[2]; };
 
 template <int DHP>
 __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_constant__ AttnCall a, uint32_t splits) {
@@ -227,7 +230,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
     static_assert(2 * kRows * (PITCH + 8) <= (4 + C::Buffers) * C::Tile, "the results fit");
     if (tid == 0) {
         for (uint32_t i = 0; i < NBUF; ++i) { mbar_init(smem_u32(&bars.full[i]), 96); mbar_init(smem_u32(&bars.empty[i]), 1); }
-        for (uint32_t i = 0; i < 2; ++i) { mbar_init(smem_u32(&bars.ready[i]), 4); mbar_init(smem_u32(&bars.done[i]), 1); }
+        for (uint32_t i = 0; i < 2; ++i) { mbar_init(smem_u32(&bars.half[i]), 4); mbar_init(smem_u32(&bars.ready[i]), 4); mbar_init(smem_u32(&bars.done[i]), 1); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kWarpMma) {
@@ -260,11 +263,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
                     mma4_ss<2, 2>(d, q + (x < DHP / 64 ? C::Tile >> 4 : 0u) + off, k + off, idesc_s, x, lead);
                 }
             };
-            auto values = [&](uint32_t w, uint32_t i) {                  // P V
+            auto values = [&](uint32_t w, uint32_t i, uint32_t half) {   // P V of 64 keys
                 const uint32_t v = desc_lo(ring + i % NBUF * C::Tile, C::Half >> 4), pt = tmem + w * kKeys, d = tmem + 2 * kKeys + w * kKeys;
 #pragma unroll 1
-                for (uint32_t x = 0; x < 4; ++x)                         // 64 keys of one part
-                    mma4_ts<16, 128>(d, pt + (x & 1u) * 64u + (x < 2 ? 8u : 0u), v + (x & 1u) * 512u, idesc_o, x, lead);
+                for (uint32_t x = 0; x < 2; ++x) mma4_ts<16, 128>(d, pt + half * 64u + (x ? 0u : 8u), v + half * 512u, idesc_o, half | x, lead);
             };
             ok = wait_full(0);
             for (uint32_t w = 0; w < tiles2 && ok; ++w) {
@@ -278,10 +280,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
             for (uint32_t j = 0; j < n && ok; ++j) {
                 const uint32_t iv = 2 * j + 1, ik = 2 * j + 2;
                 for (uint32_t w = 0; w < tiles2; ++w) {
-                    ok = wait_for(bars.ready[w], (j + 1) & 1u, &gone) && (w || wait_full(iv));
+                    if (C::Early) {
+                        ok = wait_for(bars.half[w], j & 1u, &gone) && (w || wait_full(iv));
+                        if (!ok) break;
+                        fence_after();
+                        values(w, iv, 0);
+                    }
+                    ok = wait_for(bars.ready[w], (j + 1) & 1u, &gone) && (C::Early || w || wait_full(iv));
                     if (!ok) break;
                     fence_after();
-                    values(w, iv);
+                    if (!C::Early) values(w, iv, 0);
+                    values(w, iv, 1);
                     if (w + 1 == tiles2) commit(smem_u32(&bars.empty[iv % NBUF]), lead);
                     if (j + 1 < n) {
                         if (!w && !wait_full(ik)) { ok = false; break; }
@@ -357,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
             const uint32_t first_row = row - lane, piece = lane % LR;
             float back = 1.f;
             __syncwarp();
-            constexpr uint32_t AHEAD = 16;                               // turns whose loads are on their way together
+            constexpr uint32_t AHEAD = 32 / RT;                          // all loads on their way together: nothing else is in the registers yet
             const float by = a.scale * kLog2e;
 #pragma unroll 1
             for (uint32_t i0 = 0; i0 < 32; i0 += AHEAD * RT) {
@@ -403,6 +412,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
                 for (uint32_t d = 0; d < DHP; d += 16) tmem_st(ot + d, none);
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             }
+            auto hand_over = [&](uint64_t& bar) {                        // what has been stored and read, to the issuing warp
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                fence_before();
+                __syncwarp();
+                mbar_arrive_if(smem_u32(&bar), lane == 0);
+            };
             // S of the tiles that not every row of the warp sees whole: what a row does not see is -infinity from here on
             auto hide = [&](uint32_t u0) {
                 const int p = place[row], lo = window_from(a.mask, p), sinks = (int)a.mask.sinks;
@@ -467,6 +482,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
                         parts(y[c & 1][k], y[c & 1][k + 1], x[g + (k >> 1)], x[8 + g + (k >> 1)]);
                     }
                     if (c & 1u) tmem_st(st + 8 * (c - 1), x);
+                    if (C::Early && c + 1 == N / 2) hand_over(bars.half[w]);
                 }
                 l = fmaf(l, now, (sum[0] + sum[1]) + (sum[2] + sum[3]));
             };
@@ -478,10 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
                 m = mn;
                 weights(base, now);
                 corr = now;
-                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                fence_before();
-                __syncwarp();
-                mbar_arrive_if(smem_u32(&bars.ready[w]), lane == 0);
+                hand_over(bars.ready[w]);
             }
             if (n && ok) {
                 if (wait_for(bars.done[w], n & 1u, &gone)) {
@@ -527,7 +540,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
     // ---- rows that are computed again, or whose pages were not all there ----
     float* const rows_at = reinterpret_cast<float*>(smem_dyn + (region - smem_u32(smem_dyn)));
     float2* const stats_at = reinterpret_cast<float2*>(smem_dyn + (stats - smem_u32(smem_dyn)));
-    if (warp >= 4)
+    uint32_t any = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 2 * kRows / 32; ++i) any |= odd[i];
+    if (warp >= 4 && (any || bad_page || gone))
         for (uint32_t i = warp - 4; i < rows; i += 8) {
             if (bad_page || gone) { if (lane == 0) stats_at[i].y = CUDART_NAN_F; }
             else if (odd[i >> 5] >> (i & 31u) & 1u) row_again<__half>(a, b, h, place[i], kt, t0, t1, a.q + number_of(i) * dh, rows_at + i * (PITCH / 4), stats_at + i);
