@@ -186,8 +186,9 @@ typedef struct tm_cuda_kv_pages {
 } tm_cuda_kv_pages;
 /* qkv: [T][(H + 2 KVH) * dh] fp32, the new tokens' un-rotated q | k | v. q ([T][H * dh]) receives the rotated queries; rotated keys
  * and values go into the pages (rounded once for half). rope: (cos, sin) pairs [rope_rows][dh / 2] for the pairs (j, j + dh/2) of a
- * head, or NULL for none; a position behind the table is treated as a length out of range. q must not overlap qkv. Two sequences
- * that share a page write to it in no order. */
+ * head, or NULL for none; a position behind the table is treated as a length out of range. A token whose length is out of range is
+ * not stored and its row of q is NaN; one before position 0 is not stored and its row of q is left as it is. q must not overlap qkv.
+ * Two new tokens that the table gives the same row of a page write to it in no order. */
 bool tm_cuda_kv_append_paged_dev(const tm_cuda_kv_pages* kv, const float* qkv, float* q, unsigned T, unsigned H, const float* rope,
                                  unsigned rope_rows, void* stream);
 /* out[t] = softmax(scale q k) v over the keys j that the position p of token t sees: j <= p, and with window > 0 also

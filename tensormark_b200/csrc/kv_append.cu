@@ -6,6 +6,8 @@
 // Bound: HBM, every value read once and written once: 2000 tokens of 32 / 4 heads of 64 to an fp32 cache, 31 MB, 6.2 us (5.0 TB/s, in part
 // from L2). A decode batch is bound by its trips to memory, q_begin and the lengths, then the page: 48 tokens 2.4 us in a graph. A thread
 // takes four pairs of a head (two 16-byte reads, two writes) or four values of v, and asks for them before its warp looks for the sequence.
+// A token whose position is not known, or has no angles, is not stored and leaves NaN in its row of q: the attention that follows would
+// find the length and the pages in order in the second case, and answer from what the buffers held before.
 #include "cuda_shim.h"
 #include "common.cuh"
 #include "kv_pages.cuh"
@@ -13,6 +15,7 @@
 #include "state.h"
 
 #include <cuda_fp16.h>
+#include <math_constants.h>
 
 namespace tmc {
 namespace {
@@ -41,7 +44,15 @@ __global__ void __launch_bounds__(512) kv_append_kernel(KvBatch c, const float* 
     KvSeq s;
     if (!kv_find_seq(c, t, &b, &s)) return;                     // behind the last sequence
     const int pos = s.first + (int)(t - s.q0);
-    if (s.bad || (rope && pos >= (int)rope_rows)) { note_bad_batch(status); return; }
+    if (s.bad || (rope && pos >= (int)rope_rows)) {
+        note_bad_batch(status);
+        if (turns && h < H) {
+            float* o = q + ((size_t)t * H + h) * dh + j;
+            const float4 none = make_float4(CUDART_NAN_F, CUDART_NAN_F, CUDART_NAN_F, CUDART_NAN_F);
+            store4(o, none); store4(o + half, none);
+        }
+        return;
+    }
     if (pos < 0) return;
     size_t at;
     const bool page = kv_row(c, b, (uint32_t)pos, &at);

@@ -513,6 +513,60 @@ def test_append_checks_its_arrays(cuda, torch_mod):
         assert changed[b.table[0, 2], :, 7].any() or spoil == "range"
 
 
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("spoil", ["page", "length", "range", "rope"])
+def test_tokens_without_a_position_leave_nan(cuda, torch_mod, spoil, half):
+    """A token whose length or angles are out of range: its row of q is NaN and the attention that follows is NaN there, not what the buffers held;
+    the other rows are as without it."""
+    H, KVH, dh, page = 4, 2, 64, 16
+    make = lambda: Batch(torch_mod, [1, 3, 1], [40, 50, 20], H, KVH, dh, page, half, seed=3, extra_rows=2)  # noqa: E731
+    qkv = np.random.default_rng(2).standard_normal((7, (H + 2 * KVH) * dh)).astype(np.float32)
+    good = make()
+    want, want_k, want_v = append(cuda, good, rope_table(64, dh), qkv)
+    good.d["q"].copy_(torch_mod.from_numpy(want))
+    right = good.attend(cuda)
+    b, lost, nan, stored = make(), [], [], {0, 1, 2, 3, 4}
+    if spoil == "page":
+        b.table[1, 3] = b.npages                                           # positions 48 and 49: their queries are known, their rows are not
+        stored -= {2, 3}
+    elif spoil == "length":
+        b.total = [40, b.ld * page + 1, 20]
+        nan = [1, 2, 3]
+    elif spoil == "range":
+        b.begin = np.array([0, 1, 8, 5], np.int32)                         # the second sequence's end, the third one's begin
+        lost = [1, 2, 3, 4]
+    else:
+        nan = [2, 3]                                                       # the table ends behind position 47
+    stored -= set(nan) | set(lost)
+    b.upload()
+    q, k, v = append(cuda, b, rope_table(48 if spoil == "rope" else 64, dh), qkv, want_ok=False)
+    for t in range(7):
+        if t in nan:
+            assert np.isnan(q[t]).all(), t
+        elif t in lost or t > 4:
+            assert np.all(q[t] == 7.0), t
+        else:
+            assert np.array_equal(q[t], want[t]), t
+    for t, (s, p) in enumerate([(0, 39), (1, 47), (1, 48), (1, 49), (2, 19)]):
+        at = good.table[s, p // page], slice(None), p % page
+        for mine, new, old in ((k, want_k, b.k), (v, want_v, b.v)):
+            assert np.array_equal(mine[at], (new if t in stored else old)[at]), t
+    b.d["q"].copy_(torch_mod.from_numpy(q))
+    got = b.attend(cuda, want_ok=spoil == "rope")
+    for t in range(5):
+        if t in nan or (spoil == "page" and t in (2, 3)):
+            assert np.isnan(got[t]).all(), t
+        elif t in lost:
+            assert np.all(got[t] == 7.0), t
+        elif t in (0, 4):
+            assert np.array_equal(got[t], right[t]), t
+    if spoil == "rope":                                                    # beside rows that are NaN a row is computed key by key
+        b.k, b.v = k, v
+        kk, vv = b.rows(1)
+        ref, tol = reference(q[1].reshape(1, H, dh), kk[:48], vv[:48], 47, 0, 0, 1 / np.sqrt(dh))
+        assert np.all(np.abs(got[1].reshape(1, H, dh) - ref) <= tol)
+
+
 def test_append_then_attend_captured(cuda, torch_mod):
     """A graph of append and attention, captured once, replayed for token after token with lengths that grow on the device."""
     t = torch_mod
