@@ -205,8 +205,8 @@ size_t tm_cuda_attn_window_scratch(unsigned T, unsigned H, unsigned KVH, unsigne
 bool tm_cuda_attn_window_dev(const float* q, const void* kc, const void* vc, float* scratch, size_t scratch_bytes, float* out,
                              unsigned T, unsigned pos0, unsigned H, unsigned KVH, unsigned dh, unsigned ctx, unsigned window,
                              unsigned sinks, float scale, int kv_half, void* stream);
-/* Rules on the logits x [B][ldx], V of each row, into out [B][ldo] (which may be x with the same stride, but not overlap it
- * otherwise). In this order, each where its pointers are not NULL:
+/* Rules on the logits x [B][ldx], V of each row, into out [B][ldo] (which may be x with the same stride; otherwise no row of it overlaps
+ * one of x). In this order, each where its pointers are not NULL:
  *   repeat     a token of the row's list: x > 0 ? x / repeat[b] : x * repeat[b]
  *   frequency, presence   one that occurs c > 0 times in the list behind its first n_prompt[b] entries: x -= frequency[b] * c + presence[b]
  *   bias       x[bias_ids[i]] += bias[i], for the first n_bias[b] entries (NULL: all bias_ld); of an id that is listed twice the last one

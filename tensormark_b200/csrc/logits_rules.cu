@@ -142,6 +142,19 @@ __global__ void __launch_bounds__(kThreads, 5) logits_rules_kernel(const float* 
     }
 }
 
+// Does a row of out share memory with a row of x, other than as itself? Rows whose ranges as a whole are apart are not walked.
+bool rows_meet(const float* x, size_t ldx, const float* out, size_t ldo, unsigned B, unsigned V) {
+    if (x == out && (B == 1 || ldx == ldo)) return false;
+    if (!overlap(x, ((B - 1) * ldx + V) * sizeof(float), out, ((B - 1) * ldo + V) * sizeof(float))) return false;
+    for (unsigned i = 0, k = 0; i < B && k < B;) {
+        const uintptr_t a = (uintptr_t)(x + i * ldx), b = (uintptr_t)(out + k * ldo), n = (uintptr_t)V * sizeof(float);
+        if (a + n <= b) ++i;
+        else if (b + n <= a) ++k;
+        else return true;
+    }
+    return false;
+}
+
 template <uint32_t ITEMS>
 void go(const float* x, size_t ldx, float* out, size_t ldo, unsigned B, unsigned V, const Rules& r, cudaStream_t st) {
     constexpr uint32_t SLICE = ITEMS * kThreads * kWide;
@@ -160,6 +173,7 @@ extern "C" bool tm_cuda_logits_rules_dev(const float* x, size_t ldx, float* out,
     if (!B) return true;
     if (!x || !out || !rules) return fail("logits_rules: null pointer");
     if (!V || V > 0x7fff0000u || B > 65535u || ldx < V || ldo < V) return fail("logits_rules: %u rows of %u logits in strides of %zu and %zu", B, V, ldx, ldo);
+    if (rows_meet(x, ldx, out, ldo, B, V)) return fail("logits_rules: a row of out overlaps one of x that it is not");
     const tm_cuda_logit_rules& r = *rules;
     if (r.tokens && (!r.n_tokens || !r.tokens_ld || r.tokens_ld > 0x7fffffffu)) return fail("logits_rules: a token list without lengths or stride");
     if (!r.tokens && (r.repeat || r.presence || r.frequency)) return fail("logits_rules: penalties without a token list");

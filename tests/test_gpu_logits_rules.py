@@ -170,6 +170,29 @@ def test_rows_far_apart(cuda, torch_mod):
     t.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("B,V,n_x,n_out,shift", [(3, 1000, 2000, 2000, 1000), (3, 1001, 2002, 2002, 1001), (2, 500, 1500, 500, 500), (1, 700, 700, 9000, 0), (4, 300, 300, 300, 1200)])
+def test_rows_between_rows(cuda, torch_mod, B, V, n_x, n_out, shift):
+    """out between the rows of x, behind them, or x itself with a stride that a single row does not use: taken, and right."""
+    t, rng = torch_mod, np.random.default_rng(V)
+    x, a = case(rng, B, V, 40, 6, True, V)
+    d = {n: t.from_numpy(v.view(np.int32) if v.dtype == np.uint32 else v).cuda() for n, v in a.items()}
+    r = lib.LogitRules(tokens_ld=40, bias_ld=6, mask_ld=a["mask"].shape[1], **{n: v.data_ptr() for n, v in d.items()})
+    flat = t.full((max((B - 1) * n_x, shift + (B - 1) * n_out) + V,), 7.0, device="cuda")
+    for b in range(B):
+        flat[b * n_x:b * n_x + V] = t.from_numpy(x[b]).cuda()
+    lib.check(cuda.tm_cuda_logits_rules_dev(ptr(flat), n_x, ptr(flat[shift:]), n_out, B, V, C.byref(r), stream_ptr(t)), "logits_rules")
+    t.cuda.synchronize()
+    got = flat.cpu().numpy()
+    want, tol = plain(x, V, **a)
+    for b in range(B):
+        mine = got[shift + b * n_out:shift + b * n_out + V].astype(np.float64)
+        same = ~np.isfinite(want[b])
+        with np.errstate(invalid="ignore"):
+            assert np.array_equal(mine[same], want[b][same]) and np.all((np.abs(mine - want[b]) <= tol[b]) | same)
+        if shift:
+            assert np.array_equal(got[b * n_x:b * n_x + V], x[b])
+
+
 def test_a_step_to_the_token(cuda, torch_mod):
     """Rules, then the framework's choice: the token that the plain rules' largest logit has, lowest index on ties."""
     t, rng = torch_mod, np.random.default_rng(3)

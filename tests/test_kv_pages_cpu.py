@@ -98,6 +98,16 @@ def test_rules_arguments(L):
     refused(L, L.tm_cuda_logits_rules_dev(A, 9, A, 9, 1, 9, None, None), "null")
 
 
+@pytest.mark.parametrize("x,ldx,o,ldo,B", [
+    (A, 100, A + 400, 100, 2), (A + 400, 100, A, 100, 2), (A, 100, A + 4, 100, 1), (A + 4, 100, A, 100, 1), (A, 100, A, 101, 2), (A, 200, A, 100, 2),
+    (A, 200, A + 396, 200, 3), (A, 200, A + 404, 200, 3), (A, 300, A + 400 + 4 * 250 * 9, 250, 40), (A + 4 * 99 + 2, 100, A, 100, 1),
+    (A, 1000, A + 4 * 1000 * 65534 + 396, 1000, 65535), (A + 4 * 1000 * 65534, 100, A, 1000, 65535)])
+def test_rules_where_rows_overlap(L, x, ldx, o, ldo, B):
+    """x one row behind out, another stride, a shift by less than a row: CTAs would read what others have written."""
+    r = lib.LogitRules(mask=A, mask_ld=4)
+    refused(L, L.tm_cuda_logits_rules_dev(x, ldx, o, ldo, B, 100, C.byref(r), None), "logits_rules", "overlaps")
+
+
 def test_nothing_to_do(L):
     """No tokens, no rows: a call that does nothing, with the null pointers that empty tensors have."""
     kv = pages()
