@@ -168,12 +168,12 @@ bool tm_cuda_attn_decode_static_dev(const float* q, const void* kc, const void* 
  * kv_len[b] - n .. kv_len[b] - 1 (kv_len counts them). Rows behind q_begin[B] are left as they are. Position p lies in row
  * p % page of page table[b * table_ld + p / page]; entries that no position needs may hold anything. All arrays are device memory
  * of the library's device, read when the kernels run: a captured graph may be replayed with other contents. The calls refuse what
- * the host can see. What only the device sees is checked there: a page, length or range of rows that is out of range is
- * not read or written, the rows of out that depend on it are NaN, other rows of the same sequence may be (rows that belong to no
- * sequence: left as they are), and the next synchronising entry of the lane after the kernels reports it. A new token before position 0 (more new tokens than kv_len says) is not stored,
- * and sees no key.
- * No call allocates or synchronises (the library's own first call aside: tm_cuda_init). Calls may run at the same time on several streams if each has its own scratch; a graph
- * keeps using the scratch that it was captured with. */
+ * the host can see: null pointers, sizes, boundaries, buffers of one call that overlap. What only the device sees is checked there:
+ * a page, length or range of rows that is out of range is not read or written, the rows of out that depend on it are NaN, other rows
+ * of the same sequence may be (rows that belong to no sequence: left as they are), and the next synchronising entry of the lane
+ * after the kernels reports it. A new token before position 0 (more new tokens than kv_len says) is not stored, and sees no key.
+ * No call allocates or synchronises (the library's own first call aside: tm_cuda_init). Calls may run at the same time on several
+ * streams if each has its own scratch; a graph keeps using the scratch that it was captured with. */
 typedef struct tm_cuda_kv_pages {
     void* k;                     /* [npages][KVH][page][dh], half when kv_half != 0, else fp32; on 16-byte boundaries */
     void* v;
@@ -187,15 +187,16 @@ typedef struct tm_cuda_kv_pages {
 /* qkv: [T][(H + 2 KVH) * dh] fp32, the new tokens' un-rotated q | k | v. q ([T][H * dh]) receives the rotated queries; rotated keys
  * and values go into the pages (rounded once for half). rope: (cos, sin) pairs [rope_rows][dh / 2] for the pairs (j, j + dh/2) of a
  * head, or NULL for none; a position behind the table is treated as a length out of range. A token whose length is out of range is
- * not stored and its row of q is NaN; one before position 0 is not stored and its row of q is left as it is. q must not overlap qkv.
- * Two new tokens that the table gives the same row of a page write to it in no order. */
+ * not stored and its row of q is NaN; one before position 0 is not stored and its row of q is left as it is. q, qkv and the pages
+ * must not overlap. Two new tokens that the table gives the same row of a page write to it in no order. */
 bool tm_cuda_kv_append_paged_dev(const tm_cuda_kv_pages* kv, const float* qkv, float* q, unsigned T, unsigned H, const float* rope,
                                  unsigned rope_rows, void* stream);
 /* out[t] = softmax(scale q k) v over the keys j that the position p of token t sees: j <= p, and with window > 0 also
  * j > p - window or j < sinks. A token that sees none: zeros. q, out: [T][H * dh] fp32; sums and statistics in fp32, results as from
  * fp32 products with both cache types. Values and keys that a token does not see do not count, whatever they are; where a result
- * is not finite the row is computed again key by key, which is slow. out must not overlap q. max_q: the most new tokens that one sequence has (0: not known, T); a sequence with more is
- * treated as out of range. `scratch` holds tm_cuda_attn_paged_scratch(...) bytes; what it holds before does not matter. */
+ * is not finite the row is computed again key by key, which is slow. out and scratch must not overlap each other, q or the cache.
+ * max_q: the most new tokens that one sequence has (0: not known, T); a sequence with more is treated as out of range. `scratch`
+ * holds tm_cuda_attn_paged_scratch(...) bytes; what it holds before does not matter. */
 size_t tm_cuda_attn_paged_scratch(unsigned T, unsigned B, unsigned max_q, unsigned H, unsigned KVH, unsigned dh);
 bool tm_cuda_attn_paged_dev(const tm_cuda_kv_pages* kv, const float* q, float* scratch, size_t scratch_bytes, float* out, unsigned T,
                             unsigned max_q, unsigned H, unsigned window, unsigned sinks, float scale, void* stream);

@@ -41,6 +41,14 @@ Split split(unsigned B, unsigned long long rows, unsigned rep) {
     return Split{B == 1 || rep > kFewRows ? 0u : rep <= 8 ? 8u : kFewRows, true};
 }
 
+// What a call writes, against what it reads and against each other
+bool apart(const KvBatch& c, bool half, const float* q, const float* scratch, size_t scratch_bytes, const float* out, size_t rows_bytes, const char* who) {
+    if (overlap(q, rows_bytes, out, rows_bytes)) return fail("%s: out overlaps q", who);
+    if (overlap(scratch, scratch_bytes, out, rows_bytes) || overlap(scratch, scratch_bytes, q, rows_bytes)) return fail("%s: scratch overlaps q or out", who);
+    if (overlaps_cache(c, half, out, rows_bytes) || overlaps_cache(c, half, scratch, scratch_bytes)) return fail("%s: out or scratch overlaps the cache", who);
+    return true;
+}
+
 bool launch(AttnCall a, bool half, float* scratch, cudaStream_t st) {
     const Split sp = split(a.c.B, (unsigned long long)a.max_q * a.rep, a.rep);
     a.few = sp.few; a.others = sp.others; a.status = device_status_word();
@@ -75,7 +83,7 @@ bool tm_cuda_attn_paged_dev(const tm_cuda_kv_pages* kv, const float* q, float* s
     if (!(scale > 0.f) || !std::isfinite(scale)) return fail("attn_paged: the scale is not a positive number");
     const size_t need = tm_cuda_attn_paged_scratch(T, c.B, max_q, H, c.KVH, c.dh);
     if (scratch_bytes < need) return fail("attn_paged: %zu bytes of scratch, %zu are needed", scratch_bytes, need);
-    if (overlap(q, (size_t)T * H * c.dh * 4, out, (size_t)T * H * c.dh * 4)) return fail("attn_paged: out overlaps q");
+    if (!apart(c, kv->kv_half != 0, q, scratch, need, out, (size_t)T * H * c.dh * 4, "attn_paged")) return false;
     if (!on_library_device("attn_paged")) return false;
     return launch(AttnCall{c, kv_mask(window, sinks), q, out, H, H / c.KVH, max_q && max_q < T ? max_q : T, 0, false, scale, nullptr, false}, kv->kv_half != 0, scratch, (cudaStream_t)stream);
 }
@@ -93,9 +101,9 @@ bool tm_cuda_attn_window_dev(const float* q, const void* kc, const void* vc, flo
     if (!(scale > 0.f) || !std::isfinite(scale)) return fail("attn_window: the scale is not a positive number");
     const size_t need = tm_cuda_attn_window_scratch(T, H, KVH, dh);
     if (scratch_bytes < need) return fail("attn_window: %zu bytes of scratch, %zu are needed", scratch_bytes, need);
-    if (overlap(q, (size_t)T * H * dh * 4, out, (size_t)T * H * dh * 4)) return fail("attn_window: out overlaps q");
-    if (!on_library_device("attn_window")) return false;
     const KvBatch c{kc, vc, nullptr, nullptr, nullptr, 1, KVH, dh, ctx, 1, 1, T, ctx, pos0 + T, -1};
+    if (!apart(c, kv_half != 0, q, scratch, need, out, (size_t)T * H * dh * 4, "attn_window")) return false;
+    if (!on_library_device("attn_window")) return false;
     return launch(AttnCall{c, kv_mask(window, sinks), q, out, H, H / KVH, T, 0, false, scale, nullptr, false}, kv_half != 0, scratch, (cudaStream_t)stream);
 }
 

@@ -91,12 +91,16 @@ extern "C" bool tm_cuda_kv_append_paged_dev(const tm_cuda_kv_pages* kv, const fl
     if ((uintptr_t)qkv % 16 || (uintptr_t)q % 16 || (uintptr_t)rope % 16) return fail("kv_append_paged: qkv, q and rope lie on 16-byte boundaries");
     if (rope && !rope_rows) return fail("kv_append_paged: an empty rope table");
     if (rope_rows > 0x7fffffffu) rope_rows = 0x7fffffffu;
-    if (overlap(q, (size_t)T * H * c.dh * 4, qkv, (size_t)T * (H + 2 * (size_t)c.KVH) * c.dh * 4)) return fail("kv_append_paged: q overlaps qkv");
+    const bool half = kv->kv_half != 0;
+    const size_t q_bytes = (size_t)T * H * c.dh * 4, qkv_bytes = (size_t)T * (H + 2 * (size_t)c.KVH) * c.dh * 4;
+    if (overlap(q, q_bytes, qkv, qkv_bytes)) return fail("kv_append_paged: q overlaps qkv");
+    if (overlaps_cache(c, half, q, q_bytes) || overlaps_cache(c, half, qkv, qkv_bytes)) return fail("kv_append_paged: q or qkv overlaps the cache");
+    if (overlap(c.k, kv_bytes(c, half), c.v, kv_bytes(c, half))) return fail("kv_append_paged: the pages of keys overlap those of values");
     if (!on_library_device("kv_append_paged")) return false;
     // A token's items in as few blocks as hold them, and those no larger than they need be: a token's sequence is looked for once per warp.
     const unsigned items = (H + c.KVH) * (c.dh / 8) + c.KVH * c.dh / 4, blocks = (items + 511) / 512, threads = ((items + blocks - 1) / blocks + 31) / 32 * 32;
     const dim3 grid(T, blocks);
-    launch_overlapped(kv->kv_half ? kv_append_kernel<__half> : kv_append_kernel<float>, grid, dim3(threads), 0, (cudaStream_t)stream, c, qkv, q, H, (const float2*)rope,
+    launch_overlapped(half ? kv_append_kernel<__half> : kv_append_kernel<float>, grid, dim3(threads), 0, (cudaStream_t)stream, c, qkv, q, H, (const float2*)rope,
                       rope_rows, device_status_word());
     note_launch();
     return check_launch("kv_append_paged");

@@ -120,5 +120,11 @@ constexpr float kLog2e = 1.4426950408889634f;
 bool kv_batch_from(KvBatch* c, const tm_cuda_kv_pages* kv, unsigned T, unsigned H, const char* who);
 bool on_library_device(const char* who);
 inline bool overlap(const void* a, size_t na, const void* b, size_t nb) { return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na; }
+inline size_t kv_bytes(const KvBatch& c, bool half) { return (size_t)c.npages * c.KVH * c.page * c.dh * (half ? 2 : 4); }
+// Does memory that a call writes overlap the cache or the arrays that describe it?
+inline bool overlaps_cache(const KvBatch& c, bool half, const void* a, size_t n) {
+    if (overlap(a, n, c.k, kv_bytes(c, half)) || overlap(a, n, c.v, kv_bytes(c, half))) return true;
+    return c.table && (overlap(a, n, c.table, (size_t)c.B * c.table_ld * 4) || overlap(a, n, c.q_begin, ((size_t)c.B + 1) * 4) || overlap(a, n, c.kv_len, (size_t)c.B * 4));
+}
 
 }  // namespace tmc

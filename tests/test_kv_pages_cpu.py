@@ -98,6 +98,31 @@ def test_rules_arguments(L):
     refused(L, L.tm_cuda_logits_rules_dev(A, 9, A, 9, 1, 9, None, None), "null")
 
 
+M = 1 << 24                      # buffers that are apart lie this far apart
+ROWS, POOL = 5 * 8 * 64 * 4, 9 * 2 * 16 * 64 * 2                           # bytes of q and out; of the pages that pages() describes
+
+
+@pytest.mark.parametrize("what,at", [("q", 3 * M - ROWS + 16), ("q", 3 * M + ROWS - 16), ("s", 3 * M - 16), ("s", 3 * M + ROWS - 16), ("s", M + ROWS - 16), ("o", M),
+                                     ("o", 4 * M + POOL - 16), ("o", 5 * M - ROWS + 16), ("s", 4 * M + 16), ("s", 5 * M), ("o", 6 * M + 32), ("o", 7 * M), ("s", 8 * M)])
+def test_attention_where_buffers_overlap(L, what, at):
+    """What the call writes against q, the pages, the table and the lengths."""
+    kv = pages(k=4 * M, v=5 * M, table=6 * M, q_begin=7 * M, kv_len=8 * M)
+    where = {"q": M, "s": 2 * M, "o": 3 * M, what: at}
+    need = L.tm_cuda_attn_paged_scratch(5, 3, 2, 8, 2, 64)
+    assert need > 64
+    refused(L, L.tm_cuda_attn_paged_dev(C.byref(kv), where["q"], where["s"], need, where["o"], 5, 2, 8, 0, 0, 0.1, None), "attn_paged", "overlaps")
+    if at < 6 * M and (what != "s" or at % M < 64):
+        refused(L, L.tm_cuda_attn_window_dev(where["q"], 4 * M, 5 * M, where["s"], 1 << 30, where["o"], 5, 0, 8, 2, 64, 9 * 16, 0, 0, 0.1, 1, None), "attn_window", "overlaps")
+
+
+@pytest.mark.parametrize("what,at", [("q", 4 * M + POOL - 16), ("q", 5 * M), ("x", 4 * M), ("x", 5 * M + POOL - 16), ("q", 6 * M), ("q", 7 * M), ("q", 8 * M), ("v", 4 * M + POOL - 16),
+                                     ("v", 4 * M)])
+def test_append_where_buffers_overlap(L, what, at):
+    where = {"x": M, "q": 2 * M, "v": 5 * M, what: at}
+    kv = pages(k=4 * M, v=where["v"], table=6 * M, q_begin=7 * M, kv_len=8 * M)
+    refused(L, L.tm_cuda_kv_append_paged_dev(C.byref(kv), where["x"], where["q"], 5, 8, 3 * M, 9, None), "kv_append_paged", "overlap")
+
+
 @pytest.mark.parametrize("x,ldx,o,ldo,B", [
     (A, 100, A + 400, 100, 2), (A + 400, 100, A, 100, 2), (A, 100, A + 4, 100, 1), (A + 4, 100, A, 100, 1), (A, 100, A, 101, 2), (A, 200, A, 100, 2),
     (A, 200, A + 396, 200, 3), (A, 200, A + 404, 200, 3), (A, 300, A + 400 + 4 * 250 * 9, 250, 40), (A + 4 * 99 + 2, 100, A, 100, 1),
