@@ -23,6 +23,7 @@ bool kv_batch_from(KvBatch* c, const tm_cuda_kv_pages* kv, unsigned T, unsigned 
     if (!kv->B || !kv->KVH || !kv->page || !kv->npages || !kv->table_ld) return fail("%s: a zero in the cache's description", who);
     if (!H || H % kv->KVH || H / kv->KVH > 128) return fail("%s: %u query heads for %u K/V heads (a multiple, at most 128 each)", who, H, kv->KVH);
     if (!kv->dh || kv->dh % 8 || kv->dh > 128) return fail("%s: head dimension %u (multiples of 8 up to 128)", who, kv->dh);
+    if (((uintptr_t)kv->table | (uintptr_t)kv->q_begin | (uintptr_t)kv->kv_len) % 4) return fail("%s: the table and the lengths lie on 4-byte boundaries", who);
     if ((uintptr_t)kv->k % 16 || (uintptr_t)kv->v % 16) return fail("%s: the pages lie on 16-byte boundaries", who);
     if ((unsigned long long)kv->table_ld * kv->page > 0x7fffff00ull || (unsigned long long)T * H > 0x7fffffffull || kv->B > 0x7ffffffu) return fail("%s: 2^31 positions or query rows", who);
     *c = KvBatch{kv->k, kv->v, kv->table, kv->q_begin, kv->kv_len, kv->B, kv->KVH, kv->dh, kv->page, kv->npages, kv->table_ld, T, kv->table_ld * kv->page, 0u, -1};

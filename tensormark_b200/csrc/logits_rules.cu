@@ -179,6 +179,8 @@ extern "C" bool tm_cuda_logits_rules_dev(const float* x, size_t ldx, float* out,
     if (!r.tokens && (r.repeat || r.presence || r.frequency)) return fail("logits_rules: penalties without a token list");
     if (r.bias && (!r.bias_ids || !r.bias_ld || r.bias_ld > 0x7fffffffu)) return fail("logits_rules: biases without ids or stride");
     if (r.mask && r.mask_ld < V / 32 + (V % 32 != 0)) return fail("logits_rules: a mask row of %u words for %u logits", r.mask_ld, V);
+    if (((uintptr_t)x | (uintptr_t)out | (uintptr_t)r.tokens | (uintptr_t)r.n_tokens | (uintptr_t)r.n_prompt | (uintptr_t)r.repeat | (uintptr_t)r.presence | (uintptr_t)r.frequency |
+         (uintptr_t)r.bias_ids | (uintptr_t)r.bias | (uintptr_t)r.n_bias | (uintptr_t)r.mask) % 4) return fail("logits_rules: every array lies on a 4-byte boundary");
     if (!on_library_device("logits_rules")) return false;
     const Rules k{r.tokens, r.n_tokens, r.n_prompt, r.repeat, r.presence, r.frequency, r.bias_ids, r.bias, r.n_bias, r.mask, r.tokens_ld, r.bias_ld, r.mask_ld};
     // Slices of 4096 read the lists a quarter as often, slices of 1024 spread a small batch over the SMs: 7 x 50257 takes 2.6 us with

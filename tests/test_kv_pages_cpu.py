@@ -133,6 +133,25 @@ def test_rules_where_rows_overlap(L, x, ldx, o, ldo, B):
     refused(L, L.tm_cuda_logits_rules_dev(x, ldx, o, ldo, B, 100, C.byref(r), None), "logits_rules", "overlaps")
 
 
+@pytest.mark.parametrize("name", ["table", "q_begin", "kv_len"])
+def test_batch_arrays_between_words(L, name):
+    """An address that no load of four bytes may have ends the context, so it does not get as far as a kernel."""
+    for by in (1, 2, 3):
+        kv = pages(**{name: 9 * M + by})
+        refused(L, L.tm_cuda_attn_paged_dev(C.byref(kv), 2 * M, 3 * M, 1 << 30, 4 * M, 5, 2, 8, 0, 0, 0.1, None), "attn_paged", "4-byte")
+        refused(L, L.tm_cuda_kv_append_paged_dev(C.byref(kv), 2 * M, 3 * M, 5, 8, 4 * M, 9, None), "kv_append_paged", "4-byte")
+
+
+@pytest.mark.parametrize("name", ["x", "out", "tokens", "n_tokens", "n_prompt", "repeat", "presence", "frequency", "bias_ids", "bias", "n_bias", "mask"])
+def test_rules_arrays_between_words(L, name):
+    for by in (1, 2, 3):
+        a = {n: M * (i + 1) for i, n in enumerate(["x", "out", "tokens", "n_tokens", "n_prompt", "repeat", "presence", "frequency", "bias_ids", "bias", "n_bias", "mask"])}
+        a[name] += by
+        x, out = a.pop("x"), a.pop("out")
+        r = lib.LogitRules(tokens_ld=5, bias_ld=3, mask_ld=4, **a)
+        refused(L, L.tm_cuda_logits_rules_dev(x, 100, out, 100, 2, 100, C.byref(r), None), "logits_rules", "4-byte")
+
+
 def test_nothing_to_do(L):
     """No tokens, no rows: a call that does nothing, with the null pointers that empty tensors have."""
     kv = pages()
