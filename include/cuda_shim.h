@@ -196,12 +196,13 @@ bool tm_cuda_kv_append_paged_dev(const tm_cuda_kv_pages* kv, const float* qkv, f
  * fp32 products with both cache types. Values and keys that a token does not see do not count, whatever they are; where a result
  * is not finite the row is computed again key by key, which is slow. out and scratch must not overlap each other, q or the cache.
  * max_q: the most new tokens that one sequence has (0: not known, T); a sequence with more is treated as out of range. `scratch`
- * holds tm_cuda_attn_paged_scratch(...) bytes; what it holds before does not matter. */
+ * holds tm_cuda_attn_paged_scratch(...) bytes, which are enough for calls with a smaller T, B or max_q too; what it holds before does
+ * not matter. */
 size_t tm_cuda_attn_paged_scratch(unsigned T, unsigned B, unsigned max_q, unsigned H, unsigned KVH, unsigned dh);
 bool tm_cuda_attn_paged_dev(const tm_cuda_kv_pages* kv, const float* q, float* scratch, size_t scratch_bytes, float* out, unsigned T,
                             unsigned max_q, unsigned H, unsigned window, unsigned sinks, float scale, void* stream);
 /* The same for T tokens at positions pos0 .. pos0 + T - 1 of one sequence whose caches are [KVH][ctx][dh], as
- * tm_cuda_attn_decode_dev has them; their keys and values are in the caches already. */
+ * tm_cuda_attn_decode_dev has them; their keys and values are in the caches already. Scratch for T is enough for fewer. */
 size_t tm_cuda_attn_window_scratch(unsigned T, unsigned H, unsigned KVH, unsigned dh);
 bool tm_cuda_attn_window_dev(const float* q, const void* kc, const void* vc, float* scratch, size_t scratch_bytes, float* out,
                              unsigned T, unsigned pos0, unsigned H, unsigned KVH, unsigned dh, unsigned ctx, unsigned window,

@@ -66,11 +66,11 @@ using namespace tmc;
 
 extern "C" {
 
-size_t tm_cuda_attn_paged_scratch(unsigned T, unsigned B, unsigned max_q, unsigned H, unsigned KVH, unsigned dh) {
+// What the call needs, or one with fewer tokens, sequences or new tokens of one: a prompt's call may need none, the decode step after it does.
+size_t tm_cuda_attn_paged_scratch(unsigned T, unsigned, unsigned max_q, unsigned H, unsigned KVH, unsigned dh) {
     if (!KVH || !H || H % KVH || !dh || !T) return 16;
-    const unsigned rep = H / KVH;
-    const Split sp = split(B, (unsigned long long)(max_q && max_q < T ? max_q : T) * rep, rep);
-    return sp.few ? attn_few_scratch(sp.few, dh) : 16;
+    const unsigned long long rows = (unsigned long long)(max_q && max_q < T ? max_q : T) * (H / KVH);
+    return attn_few_scratch(rows <= 8 ? 8 : kFewRows, dh);
 }
 size_t tm_cuda_attn_window_scratch(unsigned T, unsigned H, unsigned KVH, unsigned dh) { return tm_cuda_attn_paged_scratch(T, 1, T, H, KVH, dh); }
 

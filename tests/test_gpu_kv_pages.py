@@ -191,6 +191,25 @@ def test_scratch_is_enough(cuda, torch_mod, new, total, window, half):
 
 
 @pytest.mark.parametrize("half", [True, False])
+def test_one_scratch_for_a_server(cuda, torch_mod, half):
+    """Scratch for the prompts' step, then the same for chunks, drafts and single tokens of fewer sequences."""
+    t = torch_mod
+    H, KVH, dh = 8, 2, 128
+    for T, B, max_q in ((700, 1, 700), (700, 5, 600), (900, 5, 0)):
+        need = cuda.tm_cuda_attn_paged_scratch(T, B, max_q, H, KVH, dh)
+        scratch = t.full((need // 4 + 16,), 3.0, device="cuda")
+        for new, total in (([1], [4000]), ([4], [3000]), ([300], [500]), ([1] * 5, [900, 2000, 5, 77, 3100]), ([200, 1, 3], [200, 2500, 900]), ([5, 5, 4], [1800, 30, 700])):
+            if len(new) > B:
+                continue
+            b = Batch(t, new, total, H, KVH, dh, 16, half, seed=len(new))
+            out = t.full((b.T, H * dh), 7.0, device="cuda")
+            lib.check(cuda.tm_cuda_attn_paged_dev(C.byref(b.desc), ptr(b.d["q"]), ptr(scratch), need, ptr(out), b.T, max(new), H, 0, 0, 1 / np.sqrt(dh), stream_ptr(t)), "attn_paged")
+            t.cuda.synchronize()
+            b.verify(out.cpu().numpy())
+        assert bool((scratch[need // 4:] == 3.0).all())
+
+
+@pytest.mark.parametrize("half", [True, False])
 def test_offsets_past_32_bits(cuda, torch_mod, half):
     """A cache of more than 2^32 elements: pages at both of its ends, written by append and read by attention, single tokens and a chunk."""
     t, rng = torch_mod, np.random.default_rng(6)

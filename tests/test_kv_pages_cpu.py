@@ -152,6 +152,24 @@ def test_rules_arrays_between_words(L, name):
         refused(L, L.tm_cuda_logits_rules_dev(x, 100, out, 100, 2, 100, C.byref(r), None), "logits_rules", "4-byte")
 
 
+def test_scratch_of_the_largest_call_is_enough(L):
+    """A workspace made for a server's largest step serves every smaller one."""
+    sizes, out = (0, 1, 2, 3, 4, 5, 8, 9, 16, 17, 64, 1024, 1 << 20), {}
+    for H, KVH, dh in ((32, 8, 128), (8, 8, 64), (9, 3, 80), (16, 1, 128), (20, 1, 40), (128, 1, 64)):
+        for T in sizes:
+            assert L.tm_cuda_attn_window_scratch(T, H, KVH, dh) == L.tm_cuda_attn_paged_scratch(T, 1, T, H, KVH, dh)
+            for B in (1, 2, 7, 300):
+                for max_q in sizes:
+                    out[T, B, max_q] = L.tm_cuda_attn_paged_scratch(T, B, max_q, H, KVH, dh)
+                    assert out[T, B, max_q] >= 16 and out[T, B, max_q] % 16 == 0
+        for T, B, max_q in out:
+            most = max_q or T                                              # 0: not known, as many as T
+            for t in sizes:
+                for m in sizes:
+                    if t <= T and (m or t) <= most:
+                        assert all(out[t, b, m] <= out[T, B, max_q] for b in (1, 2, 7, 300) if b <= B), (T, B, max_q, t, m)
+
+
 def test_nothing_to_do(L):
     """No tokens, no rows: a call that does nothing, with the null pointers that empty tensors have."""
     kv = pages()
