@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
             // exponentials of 8 keys are under way while the 8 before them are split and stored.
             auto weights = [&](float base, float now) {
                 constexpr uint32_t N = kKeys / 8;
-                const float shift = kUp - base;
+                const float shift = kUp<__half> - base;
                 float sum[4] = {}, y[2][8];
                 uint32_t v[8], x[16], z[8];
                 tmem_ld(st, v);

@@ -14,12 +14,13 @@
 //   * Both products run on mma.sync with the query rows as its 16 rows: the keys' and values' bytes are the traffic, so the padding
 //     costs nothing that counts. Results are to be as good as fp32's, so an fp32 operand is two fp16 parts (two tf32 parts against
 //     fp32 caches), high and low: error 2^-22. With at most 8 rows the parts are the two halves of the 16 rows: one product.
-//     q is scaled by a power of two per row, and weights by 2^14, which keeps the low parts in fp16's normal range.
+//     Against fp16 caches q is scaled by a power of two per row and weights by 2^14 (kUp).
 //   * The output is summed in fp32 registers, a step's keys at a time: a tensor core's own running sum is cut, not rounded, at every step.
 //   * Over fp32 caches the same kernel takes longer chunks, 16 rows at a time (a.tiled): 700 tokens with a window of 255, 32 / 4 heads of 64,
 //     76 us, bound by the instructions that split K and V for every 16 rows.
 //   * A value that is masked for one row but not for another meets a weight of 0 in the product, which is NaN if the value is not
-//     finite. So a result that is not finite is computed again row by row, where masked keys are skipped.
+//     finite. So a result that is not finite is computed again row by row, where masked keys are skipped; one beyond 2^100, too, lest
+//     the sum of an fp32 cache's largest values be infinite where their mean is not.
 #include "attn_rows.cuh"
 #include "common.cuh"
 #include "pdl.cuh"
@@ -408,7 +409,7 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
                     corr[n] = pow2(m[n] - base);
                     m[n] = mn;
 #pragma unroll
-                    for (uint32_t i = 0; i < 2 * KB; ++i) x[i] = pow2(x[i] - base + kUp);
+                    for (uint32_t i = 0; i < 2 * KB; ++i) x[i] = pow2(x[i] - base + kUp<T>);
                     float add = x[0] + x[1];
                     if constexpr (KB == 2) add += x[2] + x[3];
                     l[n] = fmaf(l[n], corr[n], add);
@@ -509,7 +510,7 @@ __global__ void __launch_bounds__(32 * kWarps, Few<T, DHP, PAIR>::PerSm) attn_fe
                     x = fmaf(f, merge[((size_t)w * ROWS + r) * DHP + tid], x);
                     L = fmaf(f, sm_l[w][r], L);
                 }
-                again = again || !(fabsf(x) < CUDART_INF_F) || !(fabsf(L) < CUDART_INF_F);
+                again = again || !in_reach<T>(x) || !(fabsf(L) < CUDART_INF_F);
                 if (bad) L = CUDART_NAN_F;
                 if (all) {
                     a.out[number_of(u, h, r0 + r) * dh + tid] = L == 0.f ? 0.f : x / L;

@@ -8,6 +8,15 @@
 
 namespace tmc {
 
+// Partial results of a range of keys, for the merge of several: scores are kept in powers of two, and weights are 2^(s - m + kUp). Against fp16
+// caches, whose weights are split into fp16 halves, the lift keeps the high half a normal number down to 2^-28 of the largest weight and
+// the low one down to 2^-17; from there on a weight is off by up to 2^-25, 2^-39 of the largest. tf32 has fp32's exponents and needs none.
+template <typename T> constexpr float kUp = sizeof(T) == 2 ? 14.f : 0.f;
+// Sums of an fp32 cache's values beyond kFar are computed again by row_again, whose weights are 2^-kDown of the others', so that what 2^24
+// keys add up to is finite if the values are. Parts that stay below do not make the merge of 600 infinite.
+constexpr float kFar = 1.2676506e30f /* 2^100 */, kDown = 24.f;
+template <typename T> __device__ __forceinline__ bool in_reach(float x) { return fabsf(x) < (sizeof(T) == 2 ? CUDART_INF_F : kFar); }
+
 __device__ __forceinline__ float pow2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -64,9 +73,10 @@ template <uint32_t N> struct KeyTiles {
 };
 
 // One row over tiles [t0, t1) by one warp, key by key in fp32: what a kernel whose products take masked values along computes again
-// where a value was not finite. stat: the row stays unnormalised, with its maximum and sum there; nullptr: it is finished.
+// where a sum was not finite or beyond kFar. stat: the row stays unnormalised, with its maximum and sum there; nullptr: it is finished.
 template <typename T, uint32_t N>
 __device__ __noinline__ void row_again(const AttnCall& a, uint32_t b, uint32_t h, int p, KeyTiles<N> tiles, uint32_t t0, uint32_t t1, const float* q, float* to, float2* stat) {
+    constexpr float down = sizeof(T) == 2 ? 0.f : kDown, lift = sizeof(T) == 2 ? 1.f : 1.f / (1u << (int)kDown);
     const uint32_t lane = threadIdx.x & 31u, dh = a.c.dh;
     const T* kb = (const T*)a.c.k + (size_t)h * a.c.page * dh;
     const T* vb = (const T*)a.c.v + (size_t)h * a.c.page * dh;
@@ -84,7 +94,7 @@ __device__ __noinline__ void row_again(const AttnCall& a, uint32_t b, uint32_t h
                 if (lane + 32u * k < dh) x = fmaf(qr[k], (float)kb[at + lane + 32u * k], x);
 #pragma unroll
             for (int s = 16; s; s >>= 1) x += __shfl_xor_sync(0xffffffffu, x, s);
-            const float mn = fmaxf(m, x), corr = m == -CUDART_INF_F ? 0.f : exp2f(m - mn), w = x == -CUDART_INF_F ? 0.f : exp2f(x - mn + kUp);
+            const float mn = fmaxf(m, x), corr = m == -CUDART_INF_F ? 0.f : exp2f(m - mn), w = x == -CUDART_INF_F ? 0.f : lift * exp2f(x - mn + kUp<T>);
             l = fmaf(l, corr, w);
 #pragma unroll
             for (int k = 0; k < 4; ++k)
@@ -95,7 +105,7 @@ __device__ __noinline__ void row_again(const AttnCall& a, uint32_t b, uint32_t h
 #pragma unroll
     for (int k = 0; k < 4; ++k)
         if (lane + 32u * k < dh) to[lane + 32u * k] = stat ? acc[k] : l == 0.f ? 0.f : acc[k] / l;
-    if (stat && lane == 0) *stat = make_float2(m, l);
+    if (stat && lane == 0) *stat = make_float2(m + down, l);
 }
 
 }  // namespace tmc

@@ -111,9 +111,6 @@ TM_HD KvSpan kv_span(const KvMask& m, int p0, int p1) {
     return s;
 }
 
-// Partial results of a range of keys, for the merge of several: scores are kept in powers of two, and weights are 2^(s - m + kUp),
-// so that the halves into which a weight is split for the tensor cores stay in fp16's normal range down to 2^-28 of the largest.
-constexpr float kUp = 14.f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // host side (attn_pages.cu): the checks that every entry over such a batch makes; that the library is up on the current device

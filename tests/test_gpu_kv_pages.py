@@ -376,6 +376,23 @@ def test_values_over_the_range(cuda, torch_mod, half):
     b.check(cuda, scale=1e-5)
 
 
+@pytest.mark.parametrize("gain,share", [(1e-25, 1.0), (1e31, 1.0), (1e35, 1.0), (1e37, 0.02), (3.3e38, 1.0), (3.3e38, 0.02)])
+@pytest.mark.parametrize("new,total,window", [([1] * 60, [90 + 31 * i for i in range(60)], 0), ([1], [5000], 0), ([4, 4], [3000, 40], 700), ([40, 1, 33, 1], [900, 200, 33, 1], 0),
+                                              ([1, 20], [300, 1500], 130)])
+def test_values_near_the_ends_of_fp32(cuda, torch_mod, new, total, window, gain, share):
+    """An fp32 cache's values up to fp32's largest (all of them, or some keys'): a mean of them is finite, whatever the sum of so many is. Small
+    ones: products of 2^-83 and their low parts, 2^-12 and 2^-24 of that, are far from fp32's smallest normal number."""
+    b = Batch(torch_mod, new, total, 8, 2, 64, 16, False, seed=13)
+    rng = np.random.default_rng(14)
+    big = (rng.choice([-1.0, 1.0], b.v.shape) * rng.uniform(0.25, 1, b.v.shape) * gain).astype(np.float32)
+    some = rng.random(b.v.shape[:3])[..., None] < share
+    b.v = np.where(np.isnan(b.v) | ~some, b.v, big)
+    b.v[..., 7] = np.where(np.isnan(b.v[..., 7]), b.v[..., 7], np.float32(gain))       # one dim has the same value everywhere: so has its mean
+    b.upload()
+    got = b.check(cuda, window, 2)
+    assert np.isfinite(got).all()
+
+
 @pytest.mark.parametrize("rep,new", [(4, [1, 1, 1]), (4, [60, 1, 3])])
 def test_bad_arrays_are_reported(cuda, torch_mod, rep, new):
     """A page, a length and a range of rows that are not there: NaN in the rows that need them, the others right, and an error."""
