@@ -65,8 +65,9 @@ TM_HD bool kv_row(const KvBatch& c, uint32_t b, uint32_t pos, size_t* at) {
 }
 
 #ifdef __CUDACC__
+// The word is the library's one: what a wait that ran out has left there, and nobody has read yet, stays.
 __device__ __forceinline__ void note_bad_batch(int* status) {
-    if (status) *(volatile int*)status = kStatusBatch;
+    if (status && *(volatile int*)status == 0) *(volatile int*)status = kStatusBatch;
 }
 // The sequence that token t belongs to, found by a whole warp: a lane reads all there is to know of a sequence, so that one trip to memory
 // says which it is and what it is. false: none.

@@ -7,7 +7,7 @@ import ctypes as C
 import numpy as np
 import pytest
 
-from tensormark_b200 import lib
+from tensormark_b200 import lib, synth
 from tests.gpu_util import ptr, stream_ptr
 
 pytestmark = pytest.mark.gpu
@@ -428,6 +428,52 @@ def test_bad_arrays_are_reported(cuda, torch_mod, rep, new):
     b.begin[2] = 0                                                         # not ascending: which rows are left is not said, only that it is noticed
     b.upload()
     b.attend(cuda, want_ok=False)
+
+
+def test_a_wait_that_ran_out_is_reported_first(cuda, torch_mod):
+    """A batch's bad page behind a lane's wait for a rank that is not there: the next synchronising entry names the wait, whose results are lost too."""
+    t, L = torch_mod, cuda
+    n, k, dt, xs, ys, zs, st = 64, 256, synth.Q4_0, 60, 61, 62, 63
+    W, x = synth.make_weights(dt, n, k, seed=1), synth.make_activations(k, seed=2)
+    b = Batch(t, [1, 1], [40, 30], 8, 2, 64, 16, True, seed=2)
+    b.table[1, 1] = b.npages
+    b.upload()
+    need = L.tm_cuda_attn_paged_scratch(2, 2, 1, 8, 2, 64)
+    scratch, out = t.empty(need // 4 + 1, device="cuda"), t.empty(2, 8 * 64, device="cuda")
+    t.cuda.synchronize()
+    handle = (C.c_ubyte * int(L.tm_cuda_peer_handle_bytes()))()
+    assert L.tm_cuda_peer_arena(1 << 20, handle), lib.last_error()
+    prev = L.tm_cuda_set_wait_limit_ms(100)
+    try:
+        assert L.tm_cuda_peer_open_loopback(0, 2), lib.last_error()
+        assert L.tm_cuda_tok_reserve(xs, 4 * k) and L.tm_cuda_tok_reserve(zs, 4 * n) and L.tm_cuda_tok_reserve(st, 64) and L.tm_cuda_tok_reserve_shared(ys, 4 * n)
+        state, woff = np.zeros(4, np.int32), C.c_uint64(0)
+        assert L.tm_cuda_tok_upload(st, 0, state.ctypes.data, 16) and L.tm_cuda_tok_upload(xs, 0, x.ctypes.data, x.nbytes)
+        wid = L.tm_cuda_tok_wbuf(W.ctypes.data, W.nbytes, None, 0, 0, C.byref(woff))
+        assert wid >= 1000, lib.last_error()
+
+        def gemv(to, wait_site, push_site):
+            L.tm_cuda_tok_gemv_xchg(xs, 0, 0, 0, 0, None, 0.0, wid, to, (C.c_size_t * 1)(0), n, k, dt, (C.c_uint64 * 1)(woff.value), (C.c_uint * 1)(n), 1, 0,
+                                    wait_site, push_site, st)
+
+        assert L.tm_cuda_tok_begin()
+        gemv(ys, -1, 5)
+        assert L.tm_cuda_tok_flush(), lib.last_error()
+        assert L.tm_cuda_tok_begin()
+        gemv(zs, 5, -1)                                                    # for what the other rank has not pushed
+        t.cuda.synchronize()
+        lib.check(L.tm_cuda_attn_paged_dev(C.byref(b.desc), ptr(b.d["q"]), ptr(scratch), need, ptr(out), 2, 1, 8, 0, 0, 0.125, stream_ptr(t)), "attention")
+        t.cuda.synchronize()
+        assert not L.tm_cuda_tok_flush()
+        assert "bounded wait" in lib.last_error() and "status 2" in lib.last_error(), lib.last_error()
+        assert bool(t.isnan(out[1]).all()) and not bool(t.isnan(out[0]).any())
+        assert L.tm_cuda_tok_flush(), lib.last_error()
+    finally:
+        L.tm_cuda_set_wait_limit_ms(prev)
+        L.tm_cuda_peer_unmap()
+        L.tm_cuda_peer_close()
+    b.attend(cuda, want_ok=False)                                          # by itself it is what is reported
+    assert "out of range" in lib.last_error()
 
 
 def test_more_new_tokens_than_said(cuda, torch_mod):
