@@ -86,6 +86,20 @@ class Batch:
             assert np.all(off[fine] <= tol[fine]), (b, float((off / np.where(tol > 0, tol, 1)).max()), float(off.max()))
 
 
+# Root mean square of an output's error over that of the output, for values drawn independently. With relative errors e_j of the weights
+# the output is off by sum w_j e_j v_j, and sum w_j v_j is what it is, so this is the e_j's root mean square. An e_j is a score's error (in
+# powers of two, times ln 2): the dominant scores of queries of standard deviation 2 lie below 16, where a step is 2^-20. A tensor core
+# cuts its sum at dh / 16 steps (fp16; dh / 8 over fp32 caches), 0.3 of a step each at random and up to half a step alike for all large
+# scores but not for small ones, at most 8 steps of 2^-20 for 16 of them; the sums of low parts, the maximum's subtraction and ex2 add one
+# more. 9 ln 2 2^-20 < 2^-17. Weights, queries, keys or values without their low parts are off by half a step of 11 bits: 2^-11 / sqrt(3) x
+# 0.72 = 2^-12.3 (queries and keys: twice that, a score's deviation being 2), 26 times as much.
+RMS = 2.0 ** -17
+
+
+def rms_error(got, want):
+    return float(np.sqrt(np.mean((got - want) ** 2)) / np.sqrt(np.mean(want ** 2)))
+
+
 def reference(q, k, v, first, window, sinks, scale):
     """q [n, H, dh], k and v [len, KVH, dh] -> out [n, H, dh] in 64 bits, and how far an fp32-grade kernel may be from it: a score is off by its
     products' rounding (two halves of q: 2^-22, accumulation of dh products and their halves in any order: (dh + 8) roundings), at most
@@ -129,6 +143,20 @@ def test_single_tokens(cuda, torch_mod, rep, dh, half):
 def test_chunks(cuda, torch_mod, rep, dh, page, half):
     """Ragged chunks: one token to some hundred, chunks that are the whole sequence, sequences without new tokens, an empty cache."""
     Batch(torch_mod, [1, 33, 0, 7, 130], [200, 33, 50, 8, 391], 2 * rep, 2, dh, page, half, seed=page).check(cuda)
+
+
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("rep,dh,new,total", [(4, 128, [1, 1, 1], [200, 333, 2000]), (4, 64, [1, 1, 1], [77, 333, 2000]), (4, 128, [4, 3], [200, 1500]), (8, 64, [2, 2], [200, 1500]),
+                                              (16, 128, [1, 1], [333, 2000]), (4, 128, [150, 1, 70], [200, 333, 700]), (8, 64, [90, 200], [600, 200]), (1, 128, [300], [2000]),
+                                              (4, 128, [1], [5000])])
+def test_low_parts_count(cuda, torch_mod, rep, dh, new, total, half):
+    """Results as good as fp32's over a whole output: each kernel, with its low parts."""
+    b = Batch(torch_mod, new, total, 2 * rep, 2, dh, 16, half, seed=dh + rep)
+    got = b.check(cuda)
+    for s in range(b.B):
+        r = slice(b.begin[s], b.begin[s + 1])
+        want, _ = reference(b.q[r].reshape(-1, b.H, dh), *b.rows(s), total[s] - new[s], 0, 0, 1 / np.sqrt(dh))
+        assert rms_error(got[r].reshape(want.shape), want) <= RMS, (s, rms_error(got[r].reshape(want.shape), want))
 
 
 @pytest.mark.parametrize("half", [True, False])

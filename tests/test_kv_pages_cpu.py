@@ -252,3 +252,21 @@ def test_spans_cover_what_is_seen(host):
                         assert seen == any(p >= 0 and bool(host.sees(window, sinks, p, j)) for p in range(p0, p1 + 1))
                         if seen:
                             assert j < a or b <= j < e
+
+
+@pytest.mark.parametrize("dh,keys", [(64, 77), (64, 2000), (128, 200), (128, 333), (128, 2000)])
+def test_what_the_precision_bound_breaks_on(dh, keys):
+    """The bound on a whole output's error against the same attention with one operand rounded to 11 bits, in 64 bits otherwise."""
+    from tests.test_gpu_kv_pages import RMS, reference, rms_error
+    rng = np.random.default_rng(keys)
+    q, k, v = rng.standard_normal((4, 1, dh)) * 2, rng.standard_normal((keys, 1, dh)), rng.standard_normal((keys, 1, dh))
+    want, _ = reference(q, k, v, keys - 4, 0, 0, 1 / np.sqrt(dh))
+    eleven = lambda x: np.ldexp(np.round(np.ldexp(np.frexp(x)[0], 11)), np.frexp(x)[1] - 11)  # noqa: E731
+    for a in ((eleven(q), k, v), (q, eleven(k), v), (q, k, eleven(v))):
+        assert rms_error(reference(*a, keys - 4, 0, 0, 1 / np.sqrt(dh))[0], want) > 8 * RMS
+    lost = np.zeros_like(want)
+    for i in range(4):
+        s = k[:keys - 3 + i, 0] @ q[i, 0] / np.sqrt(dh)
+        w = np.exp(s - s.max())
+        lost[i, 0] = eleven(w) @ v[:keys - 3 + i, 0] / w.sum()
+    assert rms_error(lost, want) > 8 * RMS
