@@ -520,6 +520,64 @@ def test_more_new_tokens_than_said(cuda, torch_mod):
 
 
 @pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("rep,new,total", [(4, [1, 1, 1], [40, 300, 77]), (4, [60, 2, 3], [60, 300, 77]), (2, [3, 90, 70], [40, 300, 77]), (4, [40], [900]), (4, [1], [3000]), (20, [1, 33], [90, 400])])
+def test_bad_arrays_by_each_kernel(cuda, torch_mod, rep, new, total, half):
+    """A page, a length and a range of rows that are not there, in each sequence's turn: single tokens, chunks beside them, keys that a cluster shares."""
+    make = lambda: Batch(torch_mod, new, total, 2 * rep, 2, 64, 16, half, seed=2)  # noqa: E731
+    good = make()
+    for s in range(good.B):
+        rows = slice(good.begin[s], good.begin[s + 1])
+        for slot in (0, (total[s] - new[s]) // 16):                        # pages that all of the sequence's new tokens see
+            for page in (-1, good.npages, 2 ** 31 - 1, -2 ** 31):
+                b = make()
+                b.table[s, slot] = page
+                b.upload()
+                got = b.attend(cuda, want_ok=False)
+                assert "out of range" in lib.last_error() and np.isnan(got[rows]).all()
+                b.verify(got, skip=[s])
+        for length in (-1, good.ld * 16 + 1, 2 ** 31 - 1, -2 ** 31):
+            b = make()
+            b.total[s] = length
+            b.upload()
+            got = b.attend(cuda, want_ok=False)
+            assert np.isnan(got[rows]).all()
+            b.verify(got, skip=[s])
+        for begin in (-1, -2 ** 31, 2 ** 31 - 1, good.T + 1):              # of this sequence, and the end of the one before it
+            b = make()
+            b.begin[s] = begin
+            b.upload()
+            b.begin = good.begin
+            got = b.attend(cuda, want_ok=False)
+            b.verify(got, skip=[s, s - 1] if s else [s])
+            for i in {s, max(s - 1, 0)}:
+                assert np.all(got[good.begin[i]:good.begin[i + 1]] == 7.0)
+
+
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("rep,new,max_q", [(4, [1, 40, 1, 2], 10), (4, [1, 300, 10, 1], 10), (1, [17, 2, 18], 17), (2, [3, 1, 16, 8], 8), (16, [1, 2], 1), (20, [1, 5, 2], 2)])
+def test_a_broken_promise_by_each_kernel(cuda, torch_mod, rep, new, max_q, half):
+    """Sequences with more new tokens than max_q are NaN whichever kernel they would go to, all others right."""
+    total = [n + 50 + 97 * i for i, n in enumerate(new)]
+    b = Batch(torch_mod, new, total, 2 * rep, 2, 64, 16, half, seed=6, extra_rows=3)
+    long = [s for s, n in enumerate(new) if n > max_q]
+    got = b.attend(cuda, max_q=max_q, want_ok=False)
+    assert "out of range" in lib.last_error()
+    b.verify(got, skip=long)
+    for s in long:
+        assert np.isnan(got[b.begin[s]:b.begin[s + 1]]).all(), s
+    assert np.all(got[b.begin[-1]:] == 7.0)
+
+
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("new,total", [([1] * 6, [40, 300, 1, 77, 16, 2000]), ([1], [700]), ([9], [700]), ([3, 90, 1], [500, 90, 1200])])
+def test_max_q_that_is_not_known(cuda, torch_mod, new, total, half):
+    """max_q = 0: as many as T."""
+    b = Batch(torch_mod, new, total, 8, 2, 128, 16, half, seed=16, extra_rows=5)
+    b.check(cuda, max_q=0)
+    b.check(cuda, window=100, sinks=3, max_q=0)
+
+
+@pytest.mark.parametrize("half", [True, False])
 @pytest.mark.parametrize("H,KVH,dh,T,pos0,ctx,window,sinks", [
     (8, 2, 128, 1, 0, 1, 0, 0), (8, 2, 128, 1, 999, 1000, 100, 4), (32, 8, 64, 1, 4000, 4100, 1000, 4), (4, 1, 64, 200, 0, 200, 0, 0),
     (6, 2, 80, 77, 130, 300, 50, 3), (8, 2, 128, 257, 300, 600, 64, 1), (16, 1, 128, 9, 77, 100, 0, 0), (5, 5, 64, 130, 1, 200, 200, 2),
