@@ -389,6 +389,46 @@ def test_nan_and_infinity_in_masked_places(cuda, torch_mod, new, total, half):
 
 
 @pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("new,total,window", [([1, 3], [100, 700], 0), ([1], [4000], 0), ([50, 100, 1], [120, 100, 90], 60), ([1] * 70, [60 + 20 * i for i in range(70)], 0)])
+def test_infinity_in_keys_that_are_seen(cuda, torch_mod, new, total, window, half):
+    """A key of minus infinity against positive queries has no weight, whatever its value; of plus infinity, or against a query of zero, the row is NaN."""
+    b = Batch(torch_mod, new, total, 8, 2, 64, 16, half, seed=19)
+    b.q.reshape(b.T, 8, 64)[:, :, 5] = np.abs(b.q.reshape(b.T, 8, 64)[:, :, 5]) + np.float32(0.1)
+    for s, t in enumerate(total):
+        for pos in (t - 1 - (s % 7), t - 9, 3):
+            b.k[b.table[s, pos // 16], :, pos % 16, 5] = -np.inf
+    b.upload()
+    got = b.check(cuda, window, 2)
+    assert np.isfinite(got).all()
+    q, pos = b.q.reshape(b.T, 8, 64), total[-1] - 9
+    q[b.begin[1] if b.B > 1 else 0:, 2:4, 5] = 0                           # some rows of every later sequence
+    b.k[b.table[-1, pos // 16], 1, pos % 16, 9] = np.inf                   # and of the last one by the query's sign
+    b.upload()
+    b.check(cuda, window, 2)
+
+
+@pytest.mark.parametrize("half", [True, False])
+def test_many_short_sequences(cuda, torch_mod, half):
+    """More sequences than a CTA has threads, many times over: append and attention; single tokens and, beside a chunk, several launches."""
+    t, rng = torch_mod, np.random.default_rng(23)
+    for B, first in ((3000, 1), (2500, 90)):
+        new = [first] + [int(x) for x in rng.integers(0, 3, B - 1)]
+        total = [n + int(x) for n, x in zip(new, rng.integers(0, 20, B))]
+        b = Batch(t, new, total, 4, 2, 8, 4, half, seed=B, extra_rows=1)
+        b.check(cuda)
+        qkv = rng.standard_normal((b.T, (4 + 4) * 8)).astype(np.float32)
+        q, k, v = append(cuda, b, None, qkv)
+        assert np.array_equal(q[:-1], qkv[:-1, :32]) and np.all(q[-1] == 7.0)
+        kind = np.float16 if half else np.float32
+        x = qkv.reshape(b.T, 8, 8)
+        for s in range(B):
+            for i in range(new[s]):
+                pos, row = total[s] - new[s] + i, b.begin[s] + i
+                at = b.table[s, pos // 4], slice(None), pos % 4
+                assert np.array_equal(k[at], x[row, 4:6].astype(kind)) and np.array_equal(v[at], x[row, 6:].astype(kind))
+
+
+@pytest.mark.parametrize("half", [True, False])
 def test_values_over_the_range(cuda, torch_mod, half):
     """Large and small queries, keys near fp16's ends, weights that vanish: the scores decide, not the number format of the products."""
     for gain in (1e-6, 1e-2, 30.0, 1e4):
