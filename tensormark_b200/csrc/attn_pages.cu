@@ -35,7 +35,10 @@ bool kv_batch_from(KvBatch* c, const tm_cuda_kv_pages* kv, unsigned T, unsigned 
 namespace {
 
 // Which kernels serve a call: sequences with up to `few` rows per K/V head attn_few.cu, those with more (`others`: there may be some) attn_chunk.cu, or, over
-// fp32 caches, attn_few.cu again with 16 rows at a time.
+// fp32 caches, attn_few.cu again with 16 rows at a time. One launch serves all up to 16 rows. Beside longer ones `few` is 8 for groups of
+// up to 8 heads, whose single tokens then have the kernel that takes both parts in one product: 512 tokens + 16 x 1 of 32 / 8 heads of 128 in
+// fp16 112 us, with 16 for `few` 118 (+ 48 x 1: 167 and 178; fp32 815 and 852); + 16 x 4 drafted tokens, which 8 sends to 256-row tiles,
+// 157 and 126 (fp32 851 and 862). Groups of more than 16 heads have no other kernel than the tiles.
 struct Split { uint32_t few; bool others; };
 Split split(unsigned B, unsigned long long rows, unsigned rep) {
     if (rows <= kFewRows) return Split{rows <= 8 ? 8u : kFewRows, false};

@@ -19,7 +19,7 @@ struct AttnCall {
     bool tiled;                 // attn_few.cu: rows in tiles (launch_attn_tiled sets it)
 };
 
-// attn_few.cu: sequences with at most 16 query rows per K/V head
+// attn_few.cu: sequences with at most 8 or 16 query rows per K/V head (attn_pages.cu, split)
 constexpr uint32_t kChunkRows = 256, kFewRows = 16, kFewCtas = 296;       // two CTAs on each of 148 SMs
 size_t attn_few_scratch(uint32_t rows, uint32_t dh);
 bool launch_attn_few(const AttnCall& a, bool half, float* scratch, cudaStream_t st);
