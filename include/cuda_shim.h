@@ -194,8 +194,9 @@ bool tm_cuda_kv_append_paged_dev(const tm_cuda_kv_pages* kv, const float* qkv, f
 /* out[t] = softmax(scale q k) v over the keys j that the position p of token t sees: j <= p, and with window > 0 also
  * j > p - window or j < sinks. A token that sees none: zeros. q, out: [T][H * dh] fp32; sums and statistics in fp32, results as from
  * fp32 products with both cache types (over half caches a query's value is held to 2^-38 of its row's largest, a weight to 2^-39 of the
- * largest; else 22 bits of each). Values and keys that a token does not see do not count, whatever they are; where a result
- * is not finite the row is computed again key by key, which is slow. out and scratch must not overlap each other, q or the cache.
+ * largest; else 22 bits of each). Values and keys that a token does not see do not count, whatever they are; where a result is not
+ * finite, or over fp32 caches a sum of weights times values passes 2^100, the row is computed again key by key, which is slow. out and
+ * scratch must not overlap each other, q or the cache.
  * max_q: the most new tokens that one sequence has (0: not known, T); a sequence with more is treated as out of range. `scratch`
  * holds tm_cuda_attn_paged_scratch(...) bytes, which are enough for calls with a smaller T, B or max_q too; what it holds before does
  * not matter. */
